@@ -508,6 +508,38 @@ int axk_masked_attention(const void* q, const void* cache, const int32_t* block_
                          const int32_t* tiles, int n_tiles, float* partial, long partial_floats, float sink, const float* sinks,
                          int gate_per_head, int keep, int span, void* stream);
 
+// A key/value cache held in 4 bits (the format: kv4.h).  Both caches [pages][kv heads][page_size][axk_kv4_row_bytes], 16-byte
+// aligned; axk_kv4_ok: whether the kernels below take this head size (64, 128) and page size (a power of two, 8 to 1,024).
+// A token at a negative position is padding: nothing is stored for it, its rows of keys and values read back and its attention
+// are zeros.
+int axk_kv4_ok(int head_dim, int page_size);
+int axk_kv4_row_bytes(int head_dim);
+// Rotate-half on the first rotary_dim dims (a multiple of 16) of each q and k head of qkv [T][(nh + 2 nkv) hd], rows qkv_stride
+// apart: q to q_out (rows q_stride apart; qkv's own q columns are allowed), k and v quantised into the pages at each token's
+// position.  write_kv = 0: q alone, of rows that hold nh heads.  Slots of other positions are left as they were.
+int axk_rope_kv4_write(const void* qkv, long qkv_stride, void* q_out, long q_stride, const float* table, const int32_t* positions,
+                       const int32_t* seq_rows, const int32_t* block_table, int table_stride, void* k_cache, void* v_cache,
+                       int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rotary_dim, int page_size, int write_kv,
+                       void* stream);
+// Rows (seq_rows[i], positions[i]) read back: k_out and v_out [n][nkv][hd] in the compute dtype.
+int axk_kv4_read(const void* k_cache, const void* v_cache, const int32_t* block_table, int table_stride, const int32_t* positions,
+                 const int32_t* seq_rows, void* k_out, void* v_out, int n_rows, int n_kv_heads, int head_dim, int page_size,
+                 void* stream);
+// Causal attention over it; arguments, work lists and tiles as axk_attention_decode and axk_attention_prefill take them.
+int axk_kv4_decode_chunk(void);
+int axk_kv4_decode_item_factor(void);
+long axk_kv4_decode_workspace(int n_tokens, int n_heads, int head_dim, int max_chunks);
+int axk_kv4_attention_decode(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                             int table_stride, const int32_t* positions, const int32_t* seq_rows, void* out,
+                             const int32_t* token_index, int n_tokens, const int32_t* work, int n_work, float* partial,
+                             int max_chunks, int n_heads, int n_kv_heads, int head_dim, int page_size, int window, float scale,
+                             void* stream);
+int axk_kv4_prefill_tile(void);
+int axk_kv4_attention_prefill(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                              int table_stride, const int32_t* positions, const int32_t* seq_rows, void* out, const int32_t* tiles,
+                              int n_tiles, int n_heads, int n_kv_heads, int head_dim, int page_size, int window, float scale,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

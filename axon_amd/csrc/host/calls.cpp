@@ -30,7 +30,8 @@
   X(axk_softcap) X(axk_scale_rows) X(axk_add_scaled) X(axk_heads_prepare) X(axk_masked_attention_uses_mfma) \
   X(axk_masked_attention) X(axk_concat_round) X(axk_fill_i32) X(axk_fill_f32) X(axk_attention_decode_workspace) \
   X(axk_gemm_workspace) X(axk_argmax_workspace) X(axk_latent_attention_workspace) X(axk_masked_attention_workspace) \
-  X(axk_delta_chunked_workspace)
+  X(axk_delta_chunked_workspace) X(axk_kv4_ok) X(axk_kv4_row_bytes) X(axk_rope_kv4_write) X(axk_kv4_read) \
+  X(axk_kv4_decode_workspace) X(axk_kv4_attention_decode) X(axk_kv4_attention_prefill)
 
 namespace {
 

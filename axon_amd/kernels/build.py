@@ -34,7 +34,7 @@ ARCH = "gfx950"
 
 KERNEL_SOURCES = ["elementwise.hip", "gemm.hip", "gemm_mfma.hip", "attention.hip", "attention_mfma.hip", "attention_f32.hip",
                   "sampling.hip", "grouped_gemm.hip", "recurrent.hip", "state_space.hip", "time_mix.hip", "delta_rule.hip",
-                  "linear_attention.hip", "stream.hip", "latent_attention.hip", "masked_attention.hip", "moe.hip", "instances.hip",
+                  "linear_attention.hip", "stream.hip", "latent_attention.hip", "masked_attention.hip", "moe.hip", "kv4_cache.hip", "kv4_attention.hip", "instances.hip",
                   "support.hip"]
 # what a library built from a part's own kernel sources gets beside them (the error channel, the
 # list of its kernel instances)

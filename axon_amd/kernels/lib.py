@@ -176,13 +176,23 @@ _SIGNATURES = {
     "axk_concat_round": [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p],
     "axk_fill_i32": [c_void_p, c_int, c_int, c_void_p],
     "axk_fill_f32": [c_void_p, c_float, c_int, c_void_p],
+    "axk_kv4_ok": [c_int, c_int],
+    "axk_kv4_row_bytes": [c_int],
+    "axk_rope_kv4_write": [c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int,
+                           c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
+    "axk_kv4_read": [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "axk_kv4_attention_decode": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                 c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
+    "axk_kv4_attention_prefill": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                  c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
 }
 
 
 # entry points beside those of _SIGNATURES that the methods call
 _PLAIN = ["axk_argmax_workspace", "axk_attention_decode_chunk", "axk_attention_decode_item_factor", "axk_attention_decode_workspace",
           "axk_attention_prefill_tile", "axk_delta_chunked_workspace", "axk_gemm_workspace", "axk_latent_attention_workspace",
-          "axk_masked_attention_workspace", "axk_packed_elems"]
+          "axk_masked_attention_workspace", "axk_packed_elems", "axk_kv4_decode_chunk", "axk_kv4_decode_item_factor",
+          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile"]
 
 
 def _calls_module():
@@ -253,6 +263,8 @@ class Kernels:
         self.lib.axk_masked_attention_workspace.restype = ctypes.c_long
         self.lib.axk_delta_chunked_workspace.argtypes = [c_int] * 4
         self.lib.axk_delta_chunked_workspace.restype = ctypes.c_long
+        self.lib.axk_kv4_decode_workspace.argtypes = [c_int] * 4
+        self.lib.axk_kv4_decode_workspace.restype = ctypes.c_long
         self.lib.axk_packed_elems.argtypes = [c_int, c_int]
         self.lib.axk_packed_elems.restype = ctypes.c_long
         self.lib.axk_gemm_workspace.argtypes = [c_int, c_int, c_int, c_int]
@@ -329,7 +341,8 @@ class Kernels:
                   "route_topk", "route_sort", "route_combine", "gather_rows", "causal_conv", "gated_scan", "latent_prepare",
                   "latent_query_rope", "latent_attention", "heads_prepare", "masked_attention", "concat_round", "scale_rows",
                   "add_scaled", "state_conv", "state_space_scan", "gated_group_norm", "route_scored", "sum_norm", "layernorm",
-                  "softcap", "embed_pairs", "scaled_sum", "shifted_norm", "delta_low_rank", "silu_rows", "lightning_scan")
+                  "softcap", "embed_pairs", "scaled_sum", "shifted_norm", "delta_low_rank", "silu_rows", "lightning_scan", "rope_kv4_write",
+                  "kv4_read", "kv4_attention_decode", "kv4_attention_prefill")
     _MATRIX_AT = {"gemm": 1, "gemm_qkv_rope": 1, "gemm_normed_glu": 3, "gemm_normed_qkv_rope": 3, "grouped_gemm": 1}   # which argument is W
 
     def set_launch_hook(self, hook) -> None:
@@ -1651,6 +1664,178 @@ class Kernels:
             float(softcap), float(lam), float(out_scale), float(eps), _ptr(tiles), n_tiles, _ptr(partial), need,
             float("-inf") if sink is None or sinks is not None else float(sink), _ptr(sinks), 1 if gate_per_head else 0, int(keep),
             int(span), _queue()))
+        return out
+
+    # ------------------------------------------------------------------ a key/value cache held in 4 bits
+    # 32 dims of a head of one position share a scale s and a zero z (a word of 16 bits), the number held is s (n - z) with n in
+    # 0 .. 15 and |x - s (n - z)| <= s / 2, s the smallest half-precision number of six significant bits that is no less than
+    # (max(0, largest) - min(0, smallest)) / 15, at most 2,112.  4.5 bits a number.  Both caches are uint8 [pages, kv heads,
+    # page_size, kv4_row_bytes(head_dim)], what lies inside a page and head is the kernels' (csrc/kv4.h).  A token at a negative position
+    # is padding: nothing is stored for it, and its rows read back and its attention are zeros.
+    def kv4_ok(self, head_dim: int, page_size: int) -> bool:
+        """Whether the 4-bit cache's kernels take this head size (64, 128) and page size (a power of two from 8 to 1,024)."""
+        return bool(self.run.axk_kv4_ok(head_dim, page_size))
+
+    def kv4_row_bytes(self, head_dim: int) -> int:
+        """Bytes of a position's keys (or values) of one head, its scales among them."""
+        return int(self.run.axk_kv4_row_bytes(head_dim))
+
+    def _kv4_step(self, what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, *others) -> int:
+        """The checks that the 4-bit cache's calls share; the number of tokens."""
+        self._i32(positions, "positions"); self._i32(seq_rows, "seq_rows"); self._i32(block_table, "block_table")
+        if not self.kv4_ok(head_dim, page_size):
+            raise KernelError(f"{what}: head_dim {head_dim} and pages of {page_size} positions are not taken by the 4-bit cache")
+        if positions.dim() != 1 or seq_rows.shape != positions.shape or block_table.dim() != 2:
+            raise KernelError(f"{what}: positions {tuple(positions.shape)}, seq_rows {tuple(seq_rows.shape)}, block_table {tuple(block_table.shape)}")
+        here = torch.cuda.current_device()
+        if k_cache is not None:
+            shape = (n_kv_heads, page_size, self.kv4_row_bytes(head_dim))
+            for cache in (k_cache, v_cache):
+                if (cache.dtype != torch.uint8 or not cache.is_cuda or cache.dim() != 4 or tuple(cache.shape[1:]) != shape
+                        or cache.shape[0] != k_cache.shape[0] or not cache.is_contiguous()):
+                    raise KernelError(f"{what}: a cache {tuple(cache.shape)} of {cache.dtype} is not uint8 [pages, {shape[0]}, {shape[1]}, {shape[2]}]")
+        for t in (positions, seq_rows, block_table, k_cache, v_cache, *others):
+            if t is not None and t.device.index != here:
+                raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
+        return positions.numel()
+
+    def rope_kv4_write(self, qkv, q_out, table, positions, seq_rows, block_table, k_cache, v_cache, n_heads, n_kv_heads, head_dim,
+                       rotary_dim, page_size, write_kv=True) -> None:
+        """`rope_kv_write` for a cache held in 4 bits: rotate-half on the first `rotary_dim` dims (a multiple of 16) of every q and
+        k head of qkv [T, (n_heads + 2 n_kv_heads) head_dim], whose rows may lie apart; q to q_out [T, n_heads head_dim] (qkv's own
+        columns are allowed), k and v quantised from 32 bits into the pages.  Without write_kv, q alone."""
+        self._elem(qkv, "rope qkv"); self._elem(q_out, "rope q"); self._f32(table, "rope table")
+        T = self._kv4_step("rope_kv4_write", k_cache if write_kv else None, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim,
+                           page_size, qkv, q_out, table)
+        width = (n_heads + (2 * n_kv_heads if write_kv else 0)) * head_dim
+        if qkv.dim() != 2 or qkv.shape[0] != T or qkv.shape[1] < width or qkv.stride(1) != 1:
+            raise KernelError(f"rope_kv4_write: qkv {tuple(qkv.shape)} does not hold [{T}, {width}]")
+        if q_out.shape != (T, n_heads * head_dim) or q_out.stride(1) != 1 or (T > 1 and q_out.stride(0) < n_heads * head_dim):
+            raise KernelError(f"rope_kv4_write: q_out {tuple(q_out.shape)} is not [{T}, {n_heads * head_dim}]")
+        if table.shape != (T, rotary_dim // 2, 2):
+            raise KernelError(f"rope_kv4_write: table {tuple(table.shape)} for rotary_dim {rotary_dim}")
+        self._check(self.run.axk_rope_kv4_write(
+            _ptr(qkv), qkv.stride(0), _ptr(q_out), q_out.stride(0), _ptr(table), _ptr(positions), _ptr(seq_rows), _ptr(block_table),
+            block_table.shape[-1], _ptr(k_cache if write_kv else None), _ptr(v_cache if write_kv else None), T, n_heads, n_kv_heads,
+            head_dim, rotary_dim, page_size, 1 if write_kv else 0, _queue()))
+
+    def kv4_read(self, k_cache, v_cache, block_table, positions, seq_rows, k_out, v_out, n_kv_heads, head_dim, page_size) -> None:
+        """The rows of (seq_rows[i], positions[i]) out of a cache held in 4 bits: k_out, v_out [n, n_kv_heads, head_dim] of the
+        compute dtype, each number rounded once."""
+        self._elem(k_out, "kv4_read k"); self._elem(v_out, "kv4_read v")
+        n = self._kv4_step("kv4_read", k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, k_out, v_out)
+        for out in (k_out, v_out):
+            if out.shape != (n, n_kv_heads, head_dim) or not out.is_contiguous():
+                raise KernelError(f"kv4_read: rows {tuple(out.shape)} are not [{n}, {n_kv_heads}, {head_dim}]")
+        self._check(self.run.axk_kv4_read(_ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[-1], _ptr(positions),
+                                          _ptr(seq_rows), _ptr(k_out), _ptr(v_out), n, n_kv_heads, head_dim, page_size, _queue()))
+
+    @property
+    def kv4_decode_chunk(self) -> int:
+        """Positions of one item of the decoding kernel's work list (chunks lie at multiples of it)."""
+        return int(self.run.axk_kv4_decode_chunk())
+
+    @property
+    def kv4_max_context(self) -> int:
+        """The longest context that a work list can name."""
+        return self.kv4_decode_chunk * int(self.run.axk_kv4_decode_item_factor())
+
+    def _kv4_chunk_counts(self, positions, window: int):
+        pos = np.asarray(positions, dtype=np.int64)
+        lo = np.maximum(0, pos + 1 - window) if window > 0 else np.zeros_like(pos)
+        n = np.maximum(pos // self.kv4_decode_chunk - lo // self.kv4_decode_chunk + 1, 0)       # (padding: none)
+        if n.size and int(n.max()) > int(self.run.axk_kv4_decode_item_factor()):
+            raise KernelError(f"kv4_attention_decode: a context of {int(pos.max()) + 1} positions, at most {self.kv4_max_context}")
+        return n
+
+    def kv4_decode_chunks(self, positions: Sequence[int], window: int) -> int:
+        """The most chunks that any token at these positions sees (1 at least): `max_chunks` of the workspace and the call."""
+        return max(1, int(self._kv4_chunk_counts(positions, window).max(initial=0)))
+
+    def kv4_decode_work(self, positions: Sequence[int], window: int) -> List[int]:
+        """The work list of `kv4_attention_decode` for tokens at `positions` (in the order of their slots): one item per (token,
+        chunk), slot * factor + chunk counted from the token's first chunk, a token's side by side."""
+        n = self._kv4_chunk_counts(positions, window)
+        first = np.cumsum(n) - n
+        slots = np.arange(n.size, dtype=np.int64) * int(self.run.axk_kv4_decode_item_factor())
+        return (np.repeat(slots - first, n) + np.arange(int(n.sum()), dtype=np.int64)).tolist()
+
+    def kv4_decode_workspace(self, n_tokens: int, n_heads: int, head_dim: int, max_chunks: int) -> int:
+        """Floats of `partial`."""
+        return int(self.run.axk_kv4_decode_workspace(n_tokens, n_heads, head_dim, max_chunks))
+
+    def _kv4_rows(self, what, q, q_stride, out, T, n_heads, head_dim) -> None:
+        self._elem(q, what + " q"); self._elem(out, what + " out")
+        if q.dim() < 1 or q.stride(-1) != 1 or (T > 0 and q.numel() == 0):
+            raise KernelError(f"{what}: q {tuple(q.shape)}")
+        if T > 0 and (q_stride < n_heads * head_dim or q.untyped_storage().nbytes() // q.element_size() - q.storage_offset()
+                      < (T - 1) * q_stride + n_heads * head_dim):
+            raise KernelError(f"{what}: rows {q_stride} apart of q {tuple(q.shape)} do not hold {T} rows of {n_heads} heads of {head_dim}")
+        if out.dim() != 2 or tuple(out.shape) != (T, n_heads * head_dim) or not out.is_contiguous():
+            raise KernelError(f"{what}: out {tuple(out.shape)} is not [{T}, {n_heads * head_dim}]")
+
+    def kv4_attention_decode(self, q, q_stride, k_cache, v_cache, block_table, positions, seq_rows, out, token_index, partial,
+                             max_chunks, n_heads, n_kv_heads, head_dim, page_size, window, scale, work) -> torch.Tensor:
+        """`attention_decode` over a cache held in 4 bits: tokens named by token_index (int32), or the first `token_index` of the
+        step.  `work` (int32, on the device): `kv4_decode_work` of their positions, -1 for nothing; partial: float32,
+        `kv4_decode_workspace`."""
+        T = self._kv4_step("kv4_attention_decode", k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size,
+                           q, out, partial, work)
+        self._kv4_rows("kv4_attention_decode", q, q_stride, out, T, n_heads, head_dim)
+        if isinstance(token_index, int):
+            n, token_index = token_index, None
+        else:
+            self._i32(token_index, "token_index")
+            n = token_index.numel()
+        self._f32(partial, "attention partial"); self._i32(work, "attention work list")
+        if not 0 <= n <= T:
+            raise KernelError(f"kv4_attention_decode: {n} tokens of a step of {T}")
+        if max_chunks < 1 or partial.numel() < self.kv4_decode_workspace(n, n_heads, head_dim, max_chunks):
+            raise KernelError(f"kv4_attention_decode: workspace of {partial.numel()} floats is too small for {max_chunks} chunks")
+        if work.dim() != 1:
+            raise KernelError(f"kv4_attention_decode: work list {tuple(work.shape)}")
+        self._check(self.run.axk_kv4_attention_decode(
+            _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[-1], _ptr(positions), _ptr(seq_rows),
+            _ptr(out), _ptr(token_index), n, _ptr(work), work.numel(), _ptr(partial), max_chunks, n_heads, n_kv_heads, head_dim,
+            page_size, window, float(scale), _queue()))
+        return out
+
+    def kv4_prefill_tiles(self, spans, window: int, n_heads: int, n_kv_heads: int) -> List[tuple]:
+        """The tiles of `kv4_attention_prefill` for portions (first token of the step, tokens, position of the first): rows of
+        (first, count, first, count), two runs of one request's tokens that a block takes one after the other."""
+        tile = int(self.run.axk_kv4_prefill_tile())
+        runs = []
+        for start, length, at in spans:
+            if start < 0 or length < 1 or at < 0:
+                raise KernelError(f"kv4_attention_prefill: a portion of {length} tokens from token {start}, at position {at}")
+            for first in range(0, length, tile):
+                n = min(tile, length - first)
+                last = at + first + n
+                runs.append((min(last, window + n) if window > 0 else last, start + first, n))
+        runs.sort(key=lambda r: -r[0])
+        rows = []
+        for i in range((len(runs) + 1) // 2):
+            other = runs[len(runs) - 1 - i][1:] if len(runs) - 1 - i > i else (0, 0)
+            rows.append(runs[i][1:] + other)
+        return rows
+
+    def kv4_prefill_workspace(self, tiles, n_heads: int, head_dim: int) -> int:
+        """Floats of `kv4_attention_prefill`'s workspace for these tiles."""
+        return 0
+
+    def kv4_attention_prefill(self, q, q_stride, k_cache, v_cache, block_table, positions, seq_rows, out, tiles, partial, n_heads,
+                              n_kv_heads, head_dim, page_size, window, scale) -> torch.Tensor:
+        """`attention_prefill` over a cache held in 4 bits: prompt portions by `kv4_prefill_tiles` (int32 [n, 4] on the device);
+        rows of no tile are left as they are."""
+        T = self._kv4_step("kv4_attention_prefill", k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size,
+                           q, out, tiles, partial)
+        self._kv4_rows("kv4_attention_prefill", q, q_stride, out, T, n_heads, head_dim)
+        self._i32(tiles, "tiles")
+        if tiles.numel() and (tiles.dim() != 2 or tiles.shape[1] != 4):
+            raise KernelError(f"kv4_attention_prefill: tiles {tuple(tiles.shape)}")
+        self._check(self.run.axk_kv4_attention_prefill(
+            _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[-1], _ptr(positions), _ptr(seq_rows),
+            _ptr(out), _ptr(tiles), tiles.numel() // 4, n_heads, n_kv_heads, head_dim, page_size, window, float(scale), _queue()))
         return out
 
     def fill_i32(self, dst: torch.Tensor, value: int) -> None:
