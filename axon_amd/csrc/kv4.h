@@ -50,6 +50,23 @@ __device__ inline float kv4_scale_of(unsigned meta) {
   return (float)__builtin_bit_cast(_Float16, (unsigned short)(meta & 0x7FE0));
 }
 
+// A word's eight numbers as an operand of the matrix cores; s and c hold the scales and -(16 + z) s of each pair.
+__device__ __forceinline__ u32x4 kv4_operand(unsigned word, const half2_t (&s)[4], const half2_t (&c)[4]) {
+  u32x4 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned x = (__builtin_rotateright32(word, 4 * i) & 0x03C003C0u) | 0x4C004C00u;
+    out[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, x), s[i], c[i]));
+  }
+  return out;
+}
+
+// The scales of two numbers, from a pair of scale words.
+__device__ __forceinline__ void kv4_pair_scale(unsigned metas, half2_t& s, half2_t& c) {
+  s = __builtin_bit_cast(half2_t, metas & 0x7FE07FE0u);
+  c = -__builtin_bit_cast(half2_t, ((metas & 0x000F000Fu) << 6) | 0x4C004C00u) * s;
+}
+
 // One number, 32 bits.
 __device__ inline float kv4_value(unsigned n, unsigned meta) {
   return __fmul_rn(kv4_scale_of(meta), (float)((int)n - (int)(meta & 15)));

@@ -1743,14 +1743,14 @@ class Kernels:
     def _kv4_chunk_counts(self, positions, window: int):
         pos = np.asarray(positions, dtype=np.int64)
         lo = np.maximum(0, pos + 1 - window) if window > 0 else np.zeros_like(pos)
-        n = np.maximum(pos // self.kv4_decode_chunk - lo // self.kv4_decode_chunk + 1, 0)       # (padding: none)
+        n = np.maximum(pos // self.kv4_decode_chunk - lo // self.kv4_decode_chunk + 1, 1)       # (padding: one, which stores zeros)
         if n.size and int(n.max()) > int(self.run.axk_kv4_decode_item_factor()):
             raise KernelError(f"kv4_attention_decode: a context of {int(pos.max()) + 1} positions, at most {self.kv4_max_context}")
         return n
 
     def kv4_decode_chunks(self, positions: Sequence[int], window: int) -> int:
         """The most chunks that any token at these positions sees (1 at least): `max_chunks` of the workspace and the call."""
-        return max(1, int(self._kv4_chunk_counts(positions, window).max(initial=0)))
+        return int(self._kv4_chunk_counts(positions, window).max(initial=1))
 
     def kv4_decode_work(self, positions: Sequence[int], window: int) -> List[int]:
         """The work list of `kv4_attention_decode` for tokens at `positions` (in the order of their slots): one item per (token,

@@ -99,12 +99,12 @@ def pages_of(rows, page, dim, keys):
 
 def attention(q, k, v, pos, window, scale):
     """One token: q [heads, dim], k and v [positions, kv heads, dim] float64, positions 0 .. pos.  Returns the output and, for
-    bounds, sum p |v| and the largest sum_d |q_d k_d| scale of a seen position, a head."""
+    bounds, sum p |v|, the largest sum_d |q_d k_d| scale of a seen position, a head, and sum |v|, the largest max |q| sum |k_d| scale."""
     nh, dim = q.shape
     nkv = k.shape[1]
-    out, weight, score = np.zeros((nh, dim)), np.zeros((nh, dim)), np.zeros((nh, 1))
+    out, weight, score, size, spread = np.zeros((nh, dim)), np.zeros((nh, dim)), np.zeros((nh, 1)), np.zeros((nh, dim)), np.zeros((nh, 1))
     if pos < 0:
-        return out, weight, score
+        return out, weight, score, size, spread
     lo = max(0, pos + 1 - window) if window else 0
     for h in range(nh):
         kh, vh = k[lo:pos + 1, h // (nh // nkv)], v[lo:pos + 1, h // (nh // nkv)]
@@ -112,4 +112,5 @@ def attention(q, k, v, pos, window, scale):
         e = np.exp(s - s.max())
         p = e / e.sum()
         out[h], weight[h], score[h] = p @ vh, p @ np.abs(vh), (np.abs(kh) @ np.abs(q[h])).max() * scale
-    return out, weight, score
+        size[h], spread[h] = np.abs(vh).sum(0), np.abs(q[h]).max() * np.abs(kh).sum(-1).max() * scale
+    return out, weight, score, size, spread
