@@ -526,7 +526,8 @@ int axk_kv4_read(const void* k_cache, const void* v_cache, const int32_t* block_
                  const int32_t* seq_rows, void* k_out, void* v_out, int n_rows, int n_kv_heads, int head_dim, int page_size,
                  void* stream);
 // Causal attention over it; arguments, work lists and tiles as axk_attention_decode and axk_attention_prefill take them.
-int axk_kv4_decode_chunk(void);
+// A token that sees `seen` positions is cut into chunks of axk_kv4_decode_chunk(seen) positions, at multiples of that.
+int axk_kv4_decode_chunk(int seen);
 int axk_kv4_decode_item_factor(void);
 long axk_kv4_decode_workspace(int n_tokens, int n_heads, int head_dim, int max_chunks);
 int axk_kv4_attention_decode(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int32_t* block_table,

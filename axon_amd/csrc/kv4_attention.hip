@@ -13,11 +13,13 @@
 #include "instances.h"
 #include "kv4.h"
 
-#define KV4_BLOCK 64               // positions of a block: one pass of products, one maximum
-#define KV4_CHUNK 256              // positions of one item of the decoding kernel's work list
+#define KV4_BLOCK 64               // positions of a block: one pass of products
+#define KV4_WAVES 4                // waves that share a chunk, the unit of the decoding kernel's work list
+#define KV4_MOST_ROUNDS 4          // blocks of a chunk that each of them takes, at most
 #define KV4_ITEM_FACTOR 1024       // the most chunks of a token; the factor of the token's slot in an item
 #define KV4_COLUMNS 16             // query heads of a key head that a wave takes at a time
-#define KV4_SIDE_UNITS 2048        // fewer units than this: a wave a block
+#define KV4_RAISE 8.0f             // how far (log2) scores may pass the reference before it is raised
+#define KV4_WEIGHT 7.0f            // log2 of a weight at the reference: at most 2^15 goes to half precision
 #define LOG2E 1.4426950408889634f
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -53,13 +55,24 @@ __device__ __forceinline__ int kv4_query_shift(float largest) {
   return largest > 0.0f && largest < INFINITY ? 14 - ilogbf(largest) : 0;
 }
 
-// A chunk's largest score (log2), sum of weights and output, folded into what its blocks before gave.
-__device__ __forceinline__ void kv4_fold(float& m, float& l, float m_b, float l_b, float& a, float& b) {
-  const float mn = fmaxf(m, m_b), ref = mn == -INFINITY ? 0.0f : mn;
-  a = __builtin_amdgcn_exp2f(__fsub_rn(m, ref));
-  b = __builtin_amdgcn_exp2f(__fsub_rn(m_b, ref));
-  l = __builtin_fmaf(l, a, __fmul_rn(l_b, b));
-  m = mn;
+// Positions of a chunk of a token that sees `seen` positions: by the token alone, so that its result does not depend on what else a
+// step holds.  Up to 8,192 positions every wave has one block, which spreads a token over the chip; a longer one pays for
+// its partial results.  28 heads over 4 of 128, us, attention + join, one block a wave / up to four: 1 token at 8,192 5.9 + 3.4 / 11.4 + 3.0, at
+// 32,768 9.8 + 5.4 / 12.6 + 3.9; 8 tokens at 8,192 15.0 + 3.9 / 16.7 + 3.8, at 32,768 39.8 + 6.6 / 36.4 + 4.6, at 131,072 144 + 26 / 124 + 7.6.
+__host__ __device__ inline int kv4_chunk(int seen) {
+  int rounds = 1;
+  while (rounds < KV4_MOST_ROUNDS && seen > 8192 * rounds) rounds *= 2;
+  return rounds * KV4_WAVES * KV4_BLOCK;
+}
+
+// The weights are taken relative to a reference, which is raised to a block's maximum only where that is KV4_RAISE or more above it
+// (the first block's always): what was summed before is then scaled by the factor returned, 1 for a column whose
+// reference stays.  A column's arithmetic depends on its own scores alone.
+__device__ __forceinline__ float kv4_raise(float& ref, float block_max) {
+  const bool up = block_max > ref + KV4_RAISE;
+  const float before = ref;
+  ref = up ? block_max : ref;
+  return up ? __builtin_amdgcn_exp2f(__fsub_rn(before, ref)) : 1.0f;
 }
 
 // ============================================================================ single tokens
@@ -71,73 +84,110 @@ __device__ __forceinline__ void kv4_fold(float& m, float& l, float m_b, float l_
 // * V^T: row l16 of tile dt is dim HD/16 l16 + dt, so that the lane reads HD/4 neighbouring bytes of an octet, all of one group, and
 //   ends with neighbouring dims of its column.
 template <int HD>
-struct Kv4Block {                  // a block's bytes on their way: nothing of it is unpacked
-  static constexpr int KW = HD / 32, VW = HD / 64;      // words of K a row, sixteens of bytes of V^T an octet
-  unsigned k[4][KW];
-  unsigned k_scale[4];
-  uint4 v[2][VW];
-  uint4 v_scale[2];
+struct Kv4Keys {                   // a block's bytes on their way: nothing of it is unpacked
+  unsigned words[4][HD / 32], scale[4];
+};
+template <int HD>
+struct Kv4Values {
+  uint4 words[2][HD / 64], scale[2];
+};
+
+// Where a wave reads.  An octet of slots lies at the same place in both caches: its words at `words`, its scales at `scales`, in
+// units of 32 bytes from the cache's start (so 32 bits count 128 GB), each octet's in a lane.
+struct Kv4Place {
+  const unsigned char *k_words, *k_scales, *v_words, *v_scales;        // the caches' starts and the lane's part of an octet
+  unsigned words, scales;
 };
 
 template <int HD>
-__device__ __forceinline__ void kv4_load(Kv4Block<HD>& blk, const unsigned char* k_cache, const unsigned char* v_cache, int pages, int c0, int b,
-                                         size_t page_bytes, size_t head_at, int page_size, int lane) {
-  constexpr int KW = HD / 32, VW = HD / 64;
+__device__ __forceinline__ Kv4Place kv4_place_of(const unsigned char* k_cache, const unsigned char* v_cache, const int32_t* table_row, int c0,
+                                                 int pos, int wave, int kvh, int n_kv_heads, int page_size, int lane) {
+  static_assert(8 * KV4_MOST_ROUNDS <= 64, "an octet of the wave's blocks a lane");
   const int l16 = lane & 15, h = lane >> 4;
+  const int p = min(c0 + KV4_BLOCK * (KV4_WAVES * (lane >> 3) + wave) + 8 * (lane & 7), pos);      // (past the token: its own last page)
+  const unsigned page = table_row[p >> __builtin_ctz(page_size)], octet = (p & (page_size - 1)) >> 3;
+  const unsigned head = (page * n_kv_heads + kvh) * (unsigned)(page_size * kv4_row_bytes(HD) / 32);
+  Kv4Place at;
+  at.words = head + octet * (HD / 8);
+  at.scales = head + page_size * (HD / 64) + octet * (HD / 64);
+  at.k_words = k_cache + ((l16 & 3) * (HD / 2) + h * (HD / 8));
+  at.k_scales = k_cache + ((l16 & 3) * (HD / 16) + h * (HD / 4) / 32 * 2);
+  at.v_words = v_cache + l16 * (HD / 4);
+  at.v_scales = v_cache + l16 * (HD / 16) / 32 * 16;
+  return at;
+}
+
+__device__ __forceinline__ const unsigned char* kv4_at(const unsigned char* base, unsigned units) { return base + ((size_t)units << 5); }
+
+// The wave's b-th block.
+template <int HD>
+__device__ __forceinline__ void kv4_load(Kv4Keys<HD>& out, const Kv4Place& at, int b, int lane) {
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const int ko = 8 * b + 4 * u + (l16 >> 2), vo = 8 * b + 4 * u + h;      // octets of the chunk
-    const unsigned char* kp = k_cache + __shfl(pages, ko, AXON_WAVE) * page_bytes + head_at;
-    const unsigned char* vp = v_cache + __shfl(pages, vo, AXON_WAVE) * page_bytes + head_at;
-    const int k_slot = (c0 + 8 * ko) & (page_size - 1), v_octet = ((c0 + 8 * vo) & (page_size - 1)) >> 3;
+    const int octet = 8 * b + 4 * u + ((lane & 15) >> 2);
+    const unsigned char* words = kv4_at(at.k_words, __shfl(at.words, octet, AXON_WAVE));
+    const unsigned char* scales = kv4_at(at.k_scales, __shfl(at.scales, octet, AXON_WAVE));
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      const int slot = k_slot + 4 * v + (l16 & 3);
-      const unsigned char* at = kp + slot * (HD / 2) + h * (HD / 8);
-      if constexpr (KW == 4) {
-        const uint4 w = *reinterpret_cast<const uint4*>(at);
-        blk.k[2 * u + v][0] = w.x; blk.k[2 * u + v][1] = w.y; blk.k[2 * u + v][2] = w.z; blk.k[2 * u + v][3] = w.w;
+      unsigned(&w)[HD / 32] = out.words[2 * u + v];
+      if constexpr (HD == 128) {
+        const uint4 four = *reinterpret_cast<const uint4*>(words + v * 4 * (HD / 2));
+        w[0] = four.x; w[1] = four.y; w[2] = four.z; w[3] = four.w;
       } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(at);
-        blk.k[2 * u + v][0] = w.x; blk.k[2 * u + v][1] = w.y;
+        const uint2 two = *reinterpret_cast<const uint2*>(words + v * 4 * (HD / 2));
+        w[0] = two.x; w[1] = two.y;
       }
-      blk.k_scale[2 * u + v] = reinterpret_cast<const uint16_t*>(kp + page_size * (HD / 2))[slot * (HD / 32) + h * (HD / 4) / 32];
+      out.scale[2 * u + v] = *reinterpret_cast<const uint16_t*>(scales + v * 4 * (HD / 16));
     }
-    const uint4* words = reinterpret_cast<const uint4*>(vp + ((size_t)v_octet * HD + l16 * (HD / 16)) * 4);
-#pragma unroll
-    for (int i = 0; i < VW; ++i) blk.v[u][i] = words[i];
-    blk.v_scale[u] = *reinterpret_cast<const uint4*>(vp + page_size * (HD / 2) + (v_octet * (HD / 32) + l16 * (HD / 16) / 32) * 16);
   }
 }
 
-// A block's (m, l, o): o[dt][r] is dim HD/16 (4 h + r) + dt of column l16.  p0: its first position; positions lo .. pos are seen.
 template <int HD>
-__device__ __forceinline__ void kv4_block(const Kv4Block<HD>& blk, const u32x4 (&qf)[HD / 32][TERMS], int p0, int lo, int pos, float c,
-                                          int lane, float& m_b, float& l_b, f32x4 (&o)[HD / 16]) {
-  constexpr int KW = HD / 32, DT = HD / 16;
-  const int h = lane >> 4;
-  f32x4 s[4];
+__device__ __forceinline__ void kv4_load(Kv4Values<HD>& out, const Kv4Place& at, int b, int lane) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int octet = 8 * b + 4 * u + (lane >> 4);
+    const uint4* words = reinterpret_cast<const uint4*>(kv4_at(at.v_words, __shfl(at.words, octet, AXON_WAVE)));
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) out.words[u][i] = words[i];
+    out.scale[u] = *reinterpret_cast<const uint4*>(kv4_at(at.v_scales, __shfl(at.scales, octet, AXON_WAVE)));
+  }
+}
+
+// S^T of a block: s[2 u + v][r] is position 32 u + 8 h + 4 v + r of column l16, unscaled.
+template <int HD>
+__device__ __forceinline__ void kv4_scores(const Kv4Keys<HD>& keys, const u32x4 (&qf)[HD / 32][TERMS], unsigned sixteens, f32x4 (&s)[4]) {
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     half2_t sc[4], cc[4];
-    kv4_pair_scale(blk.k_scale[t] | blk.k_scale[t] << 16, sc[0], cc[0]);
+    kv4_pair_scale(keys.scale[t] | keys.scale[t] << 16, sc[0], cc[0]);
 #pragma unroll
     for (int i = 1; i < 4; ++i) { sc[i] = sc[0]; cc[i] = cc[0]; }
     s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int j = 0; j < KW; ++j) {
-      const u32x4 a = kv4_operand(blk.k[t][j], sc, cc);
+    for (int j = 0; j < HD / 32; ++j) {
+      const u32x4 a = kv4_operand(keys.words[t][j], sc, cc, sixteens);
 #pragma unroll
       for (int n = TERMS - 1; n >= 0; --n) s[t] = kv4_mma(a, qf[j][n], s[t]);
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
-  const bool whole = p0 >= lo && p0 + KV4_BLOCK - 1 <= pos;          // the same for the wave
+}
+
+// From a block's scores: its weights 2^(s c - ref + KV4_WEIGHT) as operands of O^T, added to the column's sum l.  whole: every position is
+// seen (the same for the wave); else those of lo .. pos are, and the block begins at p0.  rescale(factor) is called where a reference of
+// the wave is raised.
+template <typename Rescale>
+__device__ __forceinline__ void kv4_weights(f32x4 (&s)[4], bool whole, int p0, int lo, int pos, float c, int lane, float& ref, float& l,
+                                            u32x4 (&pf)[2][TERMS], Rescale rescale) {
   if (!whole) {
+    int first = p0 + 8 * (lane >> 4);
+    asm volatile("" : "+v"(first));            // a branch of its own: whole blocks pay nothing for the mask
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int p = p0 + 32 * (t >> 1) + 8 * h + 4 * (t & 1) + r;
+        const int p = first + 32 * (t >> 1) + 4 * (t & 1) + r;
         s[t][r] = p >= lo && p <= pos ? s[t][r] : -INFINITY;
       }
   }
@@ -148,237 +198,281 @@ __device__ __forceinline__ void kv4_block(const Kv4Block<HD>& blk, const u32x4 (
     for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
   mx = fmaxf(mx, __shfl_xor(mx, 16, AXON_WAVE));
   mx = fmaxf(mx, __shfl_xor(mx, 32, AXON_WAVE));
-  m_b = __fmul_rn(mx, c);
-  const float ref = m_b == -INFINITY ? 0.0f : __fsub_rn(14.0f, m_b);
+  const float factor = kv4_raise(ref, __fmul_rn(mx, c));
+  if (__any(factor != 1.0f)) {
+    l = __fmul_rn(l, factor);
+    rescale(factor);
+  }
+  const float add = ref == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, ref);
   float sum = 0.0f;
-  u32x4 pf[2][TERMS];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     float w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + (i >> 2)][i & 3], c, ref));
+      w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + (i >> 2)][i & 3], c, add));
       sum = __fadd_rn(sum, w[i]);
     }
     kv4_split(w, pf[u]);
   }
-  sum = __fadd_rn(sum, __shfl_xor(sum, 16, AXON_WAVE));
-  l_b = __fadd_rn(sum, __shfl_xor(sum, 32, AXON_WAVE));
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  l = __fadd_rn(l, sum);                       // (the lane's own sixteen positions of each block; the column's four lanes join at the end)
+}
+
+// The block's values, weighted, added to the column's output: o[dt][r] is dim HD/16 (4 h + r) + dt of column l16.
+template <int HD>
+__device__ __forceinline__ void kv4_values(const Kv4Values<HD>& values, const u32x4 (&pf)[2][TERMS], bool whole, int p0, int lo, int pos,
+                                           int lane, unsigned sixteens, f32x4 (&o)[HD / 16]) {
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const unsigned metas[4] = {blk.v_scale[u].x, blk.v_scale[u].y, blk.v_scale[u].z, blk.v_scale[u].w};
+    unsigned metas[4] = {values.scale[u].x, values.scale[u].y, values.scale[u].z, values.scale[u].w};
+    if (!whole) {
+      // a weight of zero times what an unseen place holds has to be zero, whatever that is
+      int first = p0 + 32 * u + 8 * (lane >> 4);
+      asm volatile("" : "+v"(first));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = first + 2 * i;
+        metas[i] &= (p >= lo && p <= pos ? 0x0000ffffu : 0u) | (p + 1 >= lo && p + 1 <= pos ? 0xffff0000u : 0u);
+      }
+    }
     half2_t sc[4], cc[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      unsigned keep = 0xffffffffu;
-      if (!whole) {
-        // a weight of zero times what an unseen place holds has to be zero, whatever that is
-        const int p = p0 + 32 * u + 8 * h + 2 * i;
-        keep = (p >= lo && p <= pos ? 0x0000ffffu : 0u) | (p + 1 >= lo && p + 1 <= pos ? 0xffff0000u : 0u);
-      }
-      kv4_pair_scale(metas[i] & keep, sc[i], cc[i]);
-    }
+    for (int i = 0; i < 4; ++i) kv4_pair_scale(metas[i], sc[i], cc[i]);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const uint4 four = blk.v[u][dt / 4];
+    for (int dt = 0; dt < HD / 16; ++dt) {
+      const uint4 four = values.words[u][dt / 4];
       const unsigned word = dt % 4 == 0 ? four.x : dt % 4 == 1 ? four.y : dt % 4 == 2 ? four.z : four.w;
-      const u32x4 a = kv4_operand(word, sc, cc);
+      const u32x4 a = kv4_operand(word, sc, cc, sixteens);
 #pragma unroll
       for (int n = TERMS - 1; n >= 0; --n) o[dt] = kv4_mma(a, pf[u][n], o[dt]);
+      if (dt % 2) __builtin_amdgcn_sched_barrier(0);       // (else every tile is unpacked before the first product)
     }
   }
 }
 
-// The wave's queries as operands: column l16 (zeros past `columns`), dims h HD/4 + 8 j + {0 .. 7}.  Returns the score's factor.
+// The wave's queries: column l16 (the last one again past `columns`), dims h HD/4 + 8 j + {0 .. 7}.
 template <int HD>
-__device__ __forceinline__ float kv4_queries(const elem_t* row, int columns, float scale, int lane, u32x4 (&qf)[HD / 32][TERMS]) {
-  constexpr int KW = HD / 32;
-  const int l16 = lane & 15, h = lane >> 4;
-  float x[KW][8], largest = 0.0f;
+struct Kv4Queries {
+  float x[HD / 32][8];
+};
+
+template <int HD>
+__device__ __forceinline__ void kv4_load(Kv4Queries<HD>& out, const elem_t* row, int columns, int lane) {
+  const elem_t* src = row + (size_t)min(lane & 15, columns - 1) * HD + (lane >> 4) * (HD / 4);
 #pragma unroll
-  for (int j = 0; j < KW; ++j) {
-    const elem_t* src = row + (size_t)min(l16, columns - 1) * HD + h * (HD / 4) + 8 * j;
+  for (int j = 0; j < HD / 32; ++j) {
     float a[4], b[4];
-    load4_guarded(src, 4, true, a);
-    load4_guarded(src + 4, 4, true, b);
+    load4_guarded(src + 8 * j, 4, true, a);
+    load4_guarded(src + 8 * j + 4, 4, true, b);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      x[j][i] = a[i];
-      x[j][4 + i] = b[i];
-      largest = fmaxf(largest, fmaxf(fabsf(a[i]), fabsf(b[i])));
+      out.x[j][i] = a[i];
+      out.x[j][4 + i] = b[i];
     }
   }
+}
+
+// As operands of S^T.  Returns the score's factor, which takes their power of two back.
+template <int HD>
+__device__ __forceinline__ float kv4_operands(Kv4Queries<HD>& q, float scale, u32x4 (&qf)[HD / 32][TERMS]) {
+  float largest = 0.0f;
+#pragma unroll
+  for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(q.x[j][i]));
   largest = fmaxf(largest, __shfl_xor(largest, 16, AXON_WAVE));
   largest = fmaxf(largest, __shfl_xor(largest, 32, AXON_WAVE));
   const int shift = kv4_query_shift(largest);
+  const float up = ldexpf(1.0f, shift / 2), up2 = ldexpf(1.0f, shift - shift / 2);      // (2^shift alone may be out of range)
 #pragma unroll
-  for (int j = 0; j < KW; ++j) {
+  for (int j = 0; j < HD / 32; ++j) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[j][i] = l16 < columns ? ldexpf(x[j][i], shift) : 0.0f;
-    kv4_split(x[j], qf[j]);
+    for (int i = 0; i < 8; ++i) q.x[j][i] = q.x[j][i] * up * up2;
+    kv4_split(q.x[j], qf[j]);
   }
   return ldexpf(scale * LOG2E, -shift);
 }
 
-// A unit is a chunk of a token and a set of up to sixteen query heads of a key head.  SIDE 1: a wave a unit, its four blocks one
-// after the other; 4: a wave a block, folded in the same order through LDS: the same bits.  Of a token of one chunk the
-// output is stored at once; else (o, m, l) go to `partial` ([slot][head][chunk][HD], then [slot][head][chunk][2]).
-template <int HD, int SIDE>
-__global__ void __launch_bounds__(64 * SIDE)
+// A workgroup has a chunk of a token and a set of up to sixteen query heads of a key head: grid (key heads x sets, work items).  Each of its
+// waves takes every KV4_WAVES-th block; what they sum is joined through LDS, in the order of the waves.  Of a token of one chunk the output
+// is stored at once; else output, reference and sum go to `partial` ([slot][head][chunk][HD], then [slot][head][chunk][2]).
+template <int HD>
+__global__ void __launch_bounds__(64 * KV4_WAVES, TERMS == 1 ? 3 : 2)
 kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned char* __restrict__ k_cache,
                   const unsigned char* __restrict__ v_cache, const int32_t* __restrict__ block_table, int table_stride,
                   const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows, elem_t* __restrict__ out,
-                  const int32_t* __restrict__ token_index, int n_tokens, const int32_t* __restrict__ work, float* __restrict__ partial,
-                  int max_chunks, int n_heads, int n_kv_heads, int sets, int page_size, int window, float scale) {
+                  const int32_t* __restrict__ token_index, int n_tokens, const int32_t* __restrict__ work, int n_work,
+                  float* __restrict__ partial, int max_chunks, int n_heads, int n_kv_heads, int sets, int page_size, int window, float scale) {
   constexpr int DT = HD / 16;
-  const int lane = threadIdx.x & 63, wave = SIDE == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per_item = n_kv_heads * sets, item = work[blockIdx.x / per_item];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, h = lane >> 4;
+  const int at_item = blockIdx.z * 65535 + blockIdx.y;
+  if (at_item >= n_work) return;
+  const int item = work[at_item];
   if (item < 0) return;                              // padding of the list
   const int slot = item / KV4_ITEM_FACTOR, chunk = item % KV4_ITEM_FACTOR;
   if (slot >= n_tokens || chunk >= max_chunks) return;
-  const int kvh = blockIdx.x % per_item / sets, set = blockIdx.x % sets;
+  const int kvh = sets == 1 ? blockIdx.x : blockIdx.x / sets, set = blockIdx.x - kvh * sets;
   const int group = n_heads / n_kv_heads, head0 = kvh * group + set * KV4_COLUMNS, columns = min(KV4_COLUMNS, group - set * KV4_COLUMNS);
   const int t = token_index ? token_index[slot] : slot, pos = positions[t];
   elem_t* out_row = out + ((size_t)t * n_heads + head0) * HD;
   if (pos < 0) {                                     // padding of the batch: zeros
     if (chunk == 0)
-      for (int i = threadIdx.x; i < columns * HD; i += 64 * SIDE) out_row[i] = from_float(0.0f);
+      for (int i = threadIdx.x; i < columns * HD; i += 64 * KV4_WAVES) out_row[i] = from_float(0.0f);
     return;
   }
-  const int lo = window > 0 ? max(0, pos + 1 - window) : 0;
-  const int first_chunk = lo / KV4_CHUNK, n_chunks = pos / KV4_CHUNK - first_chunk + 1;
+  const int lo = window > 0 ? max(0, pos + 1 - window) : 0, size = kv4_chunk(pos + 1 - lo);
+  const int first_chunk = lo / size, n_chunks = pos / size - first_chunk + 1;
   if (chunk >= n_chunks) return;
-  const int c0 = (first_chunk + chunk) * KV4_CHUNK;
-  // the pages of the chunk's 32 octets, looked up once (places past the token: its own last page)
-  const int32_t* table_row = block_table + (size_t)seq_rows[t] * table_stride;
-  const int pages = table_row[min(c0 + 8 * (lane & 31), pos) / page_size];
-  const size_t head_bytes = (size_t)page_size * kv4_row_bytes(HD), page_bytes = head_bytes * n_kv_heads, head_at = head_bytes * kvh;
-  const int b_first = max(0, lo - c0) / KV4_BLOCK, b_last = min(KV4_CHUNK - 1, pos - c0) / KV4_BLOCK;
-
-  Kv4Block<HD> blk;
-  const int b0 = SIDE == 1 ? b_first : wave;
-  if (b0 <= b_last) kv4_load<HD>(blk, k_cache, v_cache, pages, c0, b0, page_bytes, head_at, page_size, lane);
-  u32x4 qf[HD / 32][TERMS];
-  const float c = kv4_queries<HD>(q + (size_t)t * q_stride + (size_t)head0 * HD, columns, scale, lane, qf);
-  const int l16 = lane & 15, h = lane >> 4;
-  const bool alone = n_chunks == 1;
-  const size_t row = ((size_t)slot * n_heads + head0) * max_chunks + chunk;      // of column 0; a column further: max_chunks
-  float* ml = partial + (size_t)n_tokens * n_heads * max_chunks * HD;
-  if constexpr (SIDE == 1) {
-    float m = -INFINITY, l = 0.0f;
-    f32x4 acc[DT];
+  const int c0 = (first_chunk + chunk) * size;
+  // the wave's blocks: chunk blocks wave, wave + KV4_WAVES, ..., of which those from the first one that is seen to the token's own
+  const int first_block = max(0, lo - c0) / KV4_BLOCK, last_block = min(size - 1, pos - c0) / KV4_BLOCK;
+  const int b_first = max(0, first_block - wave + KV4_WAVES - 1) / KV4_WAVES, b_last = last_block < wave ? -1 : (last_block - wave) / KV4_WAVES;
+  Kv4Queries<HD> queries;
+  kv4_load<HD>(queries, q + (size_t)t * q_stride + (size_t)head0 * HD, columns, lane);
+  const Kv4Place at = kv4_place_of<HD>(k_cache, v_cache, block_table + (size_t)seq_rows[t] * table_stride, c0, pos, wave, kvh, n_kv_heads,
+                                       page_size, lane);
+  __shared__ __align__(16) float o_of[KV4_WAVES][KV4_COLUMNS][HD + 4];
+  __shared__ float ref_of[KV4_WAVES][KV4_COLUMNS], l_of[KV4_WAVES][KV4_COLUMNS];
+  float ref = -INFINITY, l = 0.0f;
+  f32x4 o[DT];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int b = b0; b <= b_last; ++b) {
-      Kv4Block<HD> next = blk;
-      if (b < b_last) kv4_load<HD>(next, k_cache, v_cache, pages, c0, b + 1, page_bytes, head_at, page_size, lane);
-      float m_b, l_b, fa, fb;
-      f32x4 o[DT];
-      kv4_block<HD>(blk, qf, c0 + b * KV4_BLOCK, lo, pos, c, lane, m_b, l_b, o);
-      kv4_fold(m, l, m_b, l_b, fa, fb);
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  if (b_first <= b_last) {
+    const unsigned sixteens = kv4_sixteens();
+    Kv4Keys<HD> keys;
+    Kv4Values<HD> values;
+    kv4_load<HD>(keys, at, b_first, lane);
+    kv4_load<HD>(values, at, b_first, lane);
+    u32x4 qf[HD / 32][TERMS];
+    const float c = kv4_operands<HD>(queries, scale, qf);
+    for (int b = b_first; b <= b_last; ++b) {
+      // the next block's keys are asked for when this one's are used up, its values likewise: each has the other's work to arrive in
+      const int p0 = c0 + (b * KV4_WAVES + wave) * KV4_BLOCK;
+      const bool whole = p0 >= lo && p0 + KV4_BLOCK - 1 <= pos;
+      f32x4 s[4];
+      u32x4 pf[2][TERMS];
+      kv4_scores<HD>(keys, qf, sixteens, s);
+      __builtin_amdgcn_sched_barrier(0);
+      if (b < b_last) kv4_load<HD>(keys, at, b + 1, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      kv4_weights(s, whole, p0, lo, pos, c, lane, ref, l, pf, [&](float factor) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[dt][r] = __builtin_fmaf(acc[dt][r], fa, __fmul_rn(o[dt][r], fb));
-      blk = next;
+          for (int r = 0; r < 4; ++r) o[dt][r] = __fmul_rn(o[dt][r], factor);
+      });
+      kv4_values<HD>(values, pf, whole, p0, lo, pos, lane, sixteens, o);
+      __builtin_amdgcn_sched_barrier(0);
+      if (b < b_last) kv4_load<HD>(values, at, b + 1, lane);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (l16 >= columns) return;
-    if (alone) {
-      const float inv = __fdiv_rn(1.0f, l);
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) out_row[l16 * HD + DT * (4 * h + r) + dt] = from_float(__fmul_rn(acc[dt][r], inv));
-      return;
-    }
-    float* dst = partial + (row + (size_t)l16 * max_chunks) * HD + DT * 4 * h;
+    l = __fadd_rn(l, __shfl_xor(l, 16, AXON_WAVE));
+    l = __fadd_rn(l, __shfl_xor(l, 32, AXON_WAVE));
+  }
+  if (l16 < columns) {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int dt = 0; dt < DT; dt += 4)
-        *reinterpret_cast<float4*>(dst + DT * r + dt) = make_float4(acc[dt][r], acc[dt + 1][r], acc[dt + 2][r], acc[dt + 3][r]);
-    if (h == 0) *reinterpret_cast<float2*>(ml + 2 * (row + (size_t)l16 * max_chunks)) = make_float2(m, l);
-  } else {
-    __shared__ __align__(16) float o_of[SIDE][KV4_COLUMNS][HD + 4];
-    __shared__ float m_of[SIDE][KV4_COLUMNS], l_of[SIDE][KV4_COLUMNS];
-    if (wave >= b_first && wave <= b_last) {
-      float m_b, l_b;
-      f32x4 o[DT];
-      kv4_block<HD>(blk, qf, c0 + wave * KV4_BLOCK, lo, pos, c, lane, m_b, l_b, o);
-      if (l16 < columns) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int dt = 0; dt < DT; dt += 4)
-            *reinterpret_cast<float4*>(&o_of[wave][l16][DT * (4 * h + r) + dt]) = make_float4(o[dt][r], o[dt + 1][r], o[dt + 2][r], o[dt + 3][r]);
-        if (h == 0) {
-          m_of[wave][l16] = m_b;
-          l_of[wave][l16] = l_b;
-        }
-      }
+        *reinterpret_cast<float4*>(&o_of[wave][l16][DT * (4 * h + r) + dt]) = make_float4(o[dt][r], o[dt + 1][r], o[dt + 2][r], o[dt + 3][r]);
+    if (h == 0) {
+      ref_of[wave][l16] = ref;
+      l_of[wave][l16] = l;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < columns * (HD / 4); i += 64 * SIDE) {
-      const int col = i / (HD / 4), d = i % (HD / 4) * 4;
-      float m = -INFINITY, l = 0.0f;
-      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int b = b_first; b <= b_last; ++b) {
-        float fa, fb;
-        kv4_fold(m, l, m_of[b][col], l_of[b][col], fa, fb);
-        const float4 o4 = *reinterpret_cast<const float4*>(&o_of[b][col][d]);
-        acc = f32x4{__builtin_fmaf(acc[0], fa, __fmul_rn(o4.x, fb)), __builtin_fmaf(acc[1], fa, __fmul_rn(o4.y, fb)),
-                    __builtin_fmaf(acc[2], fa, __fmul_rn(o4.z, fb)), __builtin_fmaf(acc[3], fa, __fmul_rn(o4.w, fb))};
-      }
-      if (alone) {
-        const float inv = __fdiv_rn(1.0f, l);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < columns * (HD / 4); i += 64 * KV4_WAVES) {
+    const int col = i / (HD / 4), d = i % (HD / 4) * 4;
+    float top = ref_of[0][col];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out_row[col * HD + d + e] = from_float(__fmul_rn(acc[e], inv));
-      } else {
-        *reinterpret_cast<float4*>(partial + (row + (size_t)col * max_chunks) * HD + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (d == 0) *reinterpret_cast<float2*>(ml + 2 * (row + (size_t)col * max_chunks)) = make_float2(m, l);
-      }
+    for (int w = 1; w < KV4_WAVES; ++w) top = fmaxf(top, ref_of[w][col]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float weight = 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < KV4_WAVES; ++w) {
+      const float f = __builtin_amdgcn_exp2f(__fsub_rn(ref_of[w][col], base));
+      const f32x4 v = *reinterpret_cast<const f32x4*>(&o_of[w][col][d]);
+      weight = __builtin_fmaf(l_of[w][col], f, weight);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = __builtin_fmaf(v[e], f, sum[e]);
+    }
+    if (n_chunks == 1) {
+      const float inv = __fdiv_rn(1.0f, weight);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out_row[col * HD + d + e] = from_float(__fmul_rn(sum[e], inv));
+    } else {
+      const size_t row = ((size_t)slot * n_heads + head0 + col) * max_chunks + chunk;
+      *reinterpret_cast<f32x4*>(partial + row * HD + d) = sum;
+      if (d == 0) *reinterpret_cast<float2*>(partial + (size_t)n_tokens * n_heads * max_chunks * HD + 2 * row) = make_float2(top, weight);
     }
   }
 }
 
-// A token's chunks joined: with M the largest of their maxima, out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M), four sums side by
-// side over every fourth chunk, ascending, added in order.  grid (tokens, heads), 4 HD threads.
+// A token's chunks joined: with M the largest of their maxima, out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M); JOIN_SUMS sums side
+// by side over every JOIN_SUMS-th chunk, ascending, added in order.  grid (tokens, heads); a thread has four dims of one of the sums.
+#define JOIN_SUMS 8
 template <int HD>
-__global__ void __launch_bounds__(4 * HD)
+__global__ void __launch_bounds__(JOIN_SUMS * HD / 4)
 kv4_join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ positions, const int32_t* __restrict__ token_index,
                 elem_t* __restrict__ out, int n_tokens, int max_chunks, int n_heads, int window) {
-  __shared__ float factor[KV4_ITEM_FACTOR], sums[4][HD], l_sums[4], wave_max[4 * HD / 64];
+  constexpr int THREADS = JOIN_SUMS * HD / 4, AHEAD = 4;
+  __shared__ float factor[KV4_ITEM_FACTOR], l_sums[JOIN_SUMS], wave_max[THREADS / 64];
+  __shared__ __align__(16) float sums[JOIN_SUMS][HD];
   const int slot = blockIdx.x, head = blockIdx.y, t = token_index ? token_index[slot] : slot, pos = positions[t];
   if (pos < 0) return;
-  const int lo = window > 0 ? max(0, pos + 1 - window) : 0, n = min(pos / KV4_CHUNK - lo / KV4_CHUNK + 1, max_chunks);
+  const int lo = window > 0 ? max(0, pos + 1 - window) : 0, size = kv4_chunk(pos + 1 - lo), n = min(pos / size - lo / size + 1, max_chunks);
   if (n == 1) return;                                // stored by the chunk's own block
   const size_t row = ((size_t)slot * n_heads + head) * max_chunks;
   const float* ml = partial + (size_t)n_tokens * n_heads * max_chunks * HD + 2 * row;
+  const int d = threadIdx.x % (HD / 4) * 4, part = threadIdx.x / (HD / 4);
+  const float* src = partial + row * HD + d;
+  // the first chunks' outputs are asked for beside the maxima (of a chunk that is not there the last one's)
+  float4 ahead[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) ahead[j] = *reinterpret_cast<const float4*>(src + (size_t)min(part + j * JOIN_SUMS, n - 1) * HD);
   float mx = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += 4 * HD) mx = fmaxf(mx, ml[2 * i]);
+  for (int i = threadIdx.x; i < n; i += THREADS) mx = fmaxf(mx, ml[2 * i]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, AXON_WAVE));
   if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x / 64] = mx;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4 * HD / 64; ++w) mx = fmaxf(mx, wave_max[w]);
+  for (int w = 0; w < THREADS / 64; ++w) mx = fmaxf(mx, wave_max[w]);
   const float ref = mx == -INFINITY ? 0.0f : mx;
-  for (int i = threadIdx.x; i < n; i += 4 * HD) factor[i] = __builtin_amdgcn_exp2f(__fsub_rn(ml[2 * i], ref));
+  for (int i = threadIdx.x; i < n; i += THREADS) factor[i] = __builtin_amdgcn_exp2f(__fsub_rn(ml[2 * i], ref));
   __syncthreads();
-  const int d = threadIdx.x % HD, part = threadIdx.x / HD;
-  float o = 0.0f, l = 0.0f;
-  for (int i = part; i < n; i += 4) o = __builtin_fmaf(partial[(row + i) * HD + d], factor[i], o);
-  if (d == 0)
-    for (int i = part; i < n; i += 4) l = __builtin_fmaf(ml[2 * i + 1], factor[i], l);
-  sums[part][d] = o;
-  if (d == 0) l_sums[part] = l;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  float l = 0.0f;
+  auto add = [&](int i, const float4& v) {
+    const float f = factor[i];
+    o = f32x4{__builtin_fmaf(v.x, f, o[0]), __builtin_fmaf(v.y, f, o[1]), __builtin_fmaf(v.z, f, o[2]), __builtin_fmaf(v.w, f, o[3])};
+  };
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (part + j * JOIN_SUMS < n) add(part + j * JOIN_SUMS, ahead[j]);
+  int i = part + AHEAD * JOIN_SUMS;
+  for (; i + (AHEAD - 1) * JOIN_SUMS < n; i += AHEAD * JOIN_SUMS) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) ahead[j] = *reinterpret_cast<const float4*>(src + (size_t)(i + j * JOIN_SUMS) * HD);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) add(i + j * JOIN_SUMS, ahead[j]);
+  }
+  for (; i < n; i += JOIN_SUMS) add(i, *reinterpret_cast<const float4*>(src + (size_t)i * HD));
+  if (d == 0) {
+    for (int c = part; c < n; c += JOIN_SUMS) l = __builtin_fmaf(ml[2 * c + 1], factor[c], l);
+    l_sums[part] = l;
+  }
+  *reinterpret_cast<f32x4*>(&sums[part][d]) = o;
   __syncthreads();
-  if (part != 0) return;
-  const float total = __fadd_rn(__fadd_rn(sums[0][d], sums[1][d]), __fadd_rn(sums[2][d], sums[3][d]));
-  const float weight = __fadd_rn(__fadd_rn(l_sums[0], l_sums[1]), __fadd_rn(l_sums[2], l_sums[3]));
-  out[((size_t)t * n_heads + head) * HD + d] = from_float(__fmul_rn(total, __fdiv_rn(1.0f, weight)));
+  if (threadIdx.x >= HD) return;
+  float total = 0.0f, weight = 0.0f;
+#pragma unroll
+  for (int s = 0; s < JOIN_SUMS; ++s) {
+    total = __fadd_rn(total, sums[s][threadIdx.x]);
+    weight = __fadd_rn(weight, l_sums[s]);
+  }
+  out[((size_t)t * n_heads + head) * HD + threadIdx.x] = from_float(__fmul_rn(total, __fdiv_rn(1.0f, weight)));
 }
 
 // ============================================================================ prompt portions
@@ -459,7 +553,8 @@ kv4_attention_kernel(const elem_t* __restrict__ q, long q_stride, const unsigned
 }
 
 // ============================================================================ entry points
-extern "C" int axk_kv4_decode_chunk(void) { return KV4_CHUNK; }
+// Positions of a chunk of a token that sees `seen` positions.
+extern "C" int axk_kv4_decode_chunk(int seen) { return kv4_chunk(seen); }
 extern "C" int axk_kv4_decode_item_factor(void) { return KV4_ITEM_FACTOR; }
 extern "C" int axk_kv4_prefill_tile(void) { return 128; }
 
@@ -488,32 +583,29 @@ extern "C" int axk_kv4_attention_decode(const void* q, int q_stride, const void*
   if (rc != 0) return rc;
   const int sets = ceil_div(n_heads / n_kv_heads, KV4_COLUMNS);
   AXK_REQUIRE(n_tokens >= 0 && n_tokens <= 1 << 20, "kv4_attention_decode: %d tokens", n_tokens);
-  AXK_REQUIRE(max_chunks >= 1 && max_chunks <= KV4_ITEM_FACTOR, "kv4_attention_decode: %d chunks of %d positions (at most %d)", max_chunks,
-              KV4_CHUNK, KV4_ITEM_FACTOR);
-  AXK_REQUIRE(n_work >= 0 && (n_work == 0 || work != nullptr) && (long)n_work * n_kv_heads * sets < (1l << 31),
-              "kv4_attention_decode: a work list of %d items", n_work);
+  AXK_REQUIRE(max_chunks >= 1 && max_chunks <= KV4_ITEM_FACTOR, "kv4_attention_decode: %d chunks of a token (at most %d)", max_chunks,
+              KV4_ITEM_FACTOR);
+  AXK_REQUIRE(n_work >= 0 && (n_work == 0 || work != nullptr), "kv4_attention_decode: a work list of %d items", n_work);
   AXK_REQUIRE(partial != nullptr && (uintptr_t)partial % 16 == 0, "kv4_attention_decode: needs its workspace, 16-byte aligned");
   if (n_tokens == 0 || n_work == 0) return 0;
-  const unsigned units = (unsigned)n_work * n_kv_heads * sets;
-  const bool side = units < KV4_SIDE_UNITS;
-#define LAUNCH(HD, SIDE)                                                                                                        \
+  const dim3 units(n_kv_heads * sets, n_work < 65535 ? n_work : 65535, (n_work + 65534) / 65535);
+#define LAUNCH(HD)                                                                                                              \
   {                                                                                                                             \
-    AXK_INSTANCE(INST_KV4_DECODE, HD, SIDE);                                                                                    \
-    kv4_decode_kernel<HD, SIDE><<<units, 64 * SIDE, 0, (hipStream_t)stream>>>(                                                  \
+    AXK_INSTANCE(INST_KV4_DECODE, HD);                                                                                          \
+    kv4_decode_kernel<HD><<<units, 64 * KV4_WAVES, 0, (hipStream_t)stream>>>(                                                               \
         (const elem_t*)q, q_stride, (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride,    \
-        positions, seq_rows, (elem_t*)out, token_index, n_tokens, work, partial, max_chunks, n_heads, n_kv_heads, sets,         \
+        positions, seq_rows, (elem_t*)out, token_index, n_tokens, work, n_work, partial, max_chunks, n_heads, n_kv_heads, sets, \
         page_size, window, scale);                                                                                              \
   }
-  if (head_dim == 64) { if (side) LAUNCH(64, 4) else LAUNCH(64, 1) }
-  else { if (side) LAUNCH(128, 4) else LAUNCH(128, 1) }
+  if (head_dim == 64) LAUNCH(64) else LAUNCH(128)
 #undef LAUNCH
   AXK_LAUNCH_CHECK("kv4_attention_decode");
   if (max_chunks > 1) {
     if (head_dim == 64)
-      kv4_join_kernel<64><<<dim3(n_tokens, n_heads), 256, 0, (hipStream_t)stream>>>(partial, positions, token_index, (elem_t*)out, n_tokens,
+      kv4_join_kernel<64><<<dim3(n_tokens, n_heads), JOIN_SUMS * 16, 0, (hipStream_t)stream>>>(partial, positions, token_index, (elem_t*)out, n_tokens,
                                                                                     max_chunks, n_heads, window);
     else
-      kv4_join_kernel<128><<<dim3(n_tokens, n_heads), 512, 0, (hipStream_t)stream>>>(partial, positions, token_index, (elem_t*)out,
+      kv4_join_kernel<128><<<dim3(n_tokens, n_heads), JOIN_SUMS * 32, 0, (hipStream_t)stream>>>(partial, positions, token_index, (elem_t*)out,
                                                                                      n_tokens, max_chunks, n_heads, window);
     AXK_LAUNCH_CHECK("kv4_attention_decode");
   }

@@ -281,6 +281,7 @@ class Kernels:
         self.run = self._callables()
         self._extensions: Dict[str, ctypes.CDLL] = {}      # a registered source's path -> its library
         self._chunk_factor = None
+        self._kv4_steps = None
 
     def _callables(self):
         """The library's entry points as the methods call them: bound natively where that module is there (csrc/host/calls.cpp), else
@@ -1694,6 +1695,8 @@ class Kernels:
                 if (cache.dtype != torch.uint8 or not cache.is_cuda or cache.dim() != 4 or tuple(cache.shape[1:]) != shape
                         or cache.shape[0] != k_cache.shape[0] or not cache.is_contiguous()):
                     raise KernelError(f"{what}: a cache {tuple(cache.shape)} of {cache.dtype} is not uint8 [pages, {shape[0]}, {shape[1]}, {shape[2]}]")
+            if k_cache.numel() > 1 << 37:                    # places in it are 32-bit numbers of 32 bytes
+                raise KernelError(f"{what}: a cache of {k_cache.numel()} bytes, at most {1 << 37}")
         for t in (positions, seq_rows, block_table, k_cache, v_cache, *others):
             if t is not None and t.device.index != here:
                 raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
@@ -1730,20 +1733,32 @@ class Kernels:
         self._check(self.run.axk_kv4_read(_ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[-1], _ptr(positions),
                                           _ptr(seq_rows), _ptr(k_out), _ptr(v_out), n, n_kv_heads, head_dim, page_size, _queue()))
 
-    @property
-    def kv4_decode_chunk(self) -> int:
-        """Positions of one item of the decoding kernel's work list (chunks lie at multiples of it)."""
-        return int(self.run.axk_kv4_decode_chunk())
+    def _kv4_chunk_sizes(self, seen):
+        """Positions of a chunk for tokens that see so many (the kernel's rule: it grows with them, up to its largest)."""
+        if self._kv4_steps is None:
+            # where the rule steps up, and to what: (seen, size) ascending
+            steps, at, largest = [(1, int(self.run.axk_kv4_decode_chunk(1)))], 1, int(self.run.axk_kv4_decode_chunk(2 ** 30))
+            while steps[-1][1] < largest:
+                low, high = at, 2 ** 30                       # the smallest `seen` with a larger size
+                while high - low > 1:
+                    mid = (low + high) // 2
+                    low, high = (mid, high) if int(self.run.axk_kv4_decode_chunk(mid)) == steps[-1][1] else (low, mid)
+                at = high
+                steps.append((at, int(self.run.axk_kv4_decode_chunk(at))))
+            self._kv4_steps = (np.array([s for s, _ in steps]), np.array([n for _, n in steps]))
+        starts, sizes = self._kv4_steps
+        return sizes[np.searchsorted(starts, np.maximum(seen, 1), side="right") - 1]
 
     @property
     def kv4_max_context(self) -> int:
         """The longest context that a work list can name."""
-        return self.kv4_decode_chunk * int(self.run.axk_kv4_decode_item_factor())
+        return int(self._kv4_chunk_sizes(2 ** 29)) * int(self.run.axk_kv4_decode_item_factor())
 
     def _kv4_chunk_counts(self, positions, window: int):
         pos = np.asarray(positions, dtype=np.int64)
         lo = np.maximum(0, pos + 1 - window) if window > 0 else np.zeros_like(pos)
-        n = np.maximum(pos // self.kv4_decode_chunk - lo // self.kv4_decode_chunk + 1, 1)       # (padding: one, which stores zeros)
+        size = self._kv4_chunk_sizes(pos + 1 - lo)
+        n = np.maximum(pos // size - lo // size + 1, 1)       # (padding: one, which stores zeros)
         if n.size and int(n.max()) > int(self.run.axk_kv4_decode_item_factor()):
             raise KernelError(f"kv4_attention_decode: a context of {int(pos.max()) + 1} positions, at most {self.kv4_max_context}")
         return n

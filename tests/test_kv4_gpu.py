@@ -6,8 +6,8 @@ Attention's tolerance, an output o = sum p_j v_j against float64 over the same (
   float32 build three such terms, whose rest is below 2^-24;
 * scores in 32 bits: a sum of `dim` products, at most (dim + 8) 2^-24 of sum |q k| scale, which moves a weight by that much of itself,
   weights and their sum both: twice;
-* half precision's smallest step is 2^-24.  A weight is scaled by 2^14 there, so what is lost of it below that step is at most 2^-25-14 of
-  the largest weight, which is at most their sum: 2^-39 sum |v| of an output.  A query's largest number is 2^14 at least there: what is
+* half precision's smallest step is 2^-24.  Weights are 2^7 there at a reference that is no larger than a chunk's largest, so what is lost
+  of one below that step is at most 2^-25-7 of the largest, which is at most their sum: 2^-32 sum |v| of an output.  A query's largest number is 2^14 at least there: what is
   lost of the others is at most 2^-39 max |q|, of a score 2^-39 max |q| sum |k| scale;
 * the exponential and the multiply-add before it: 2^-20 of a weight;
 * sums over positions in 32 bits: blocks of 64, then a fold a block: (64 + blocks) 2^-24 of sum p |v|, numerator and denominator."""
@@ -217,7 +217,7 @@ def tolerance(dtype, want, weight, score, size, spread, dim, positions):
     eps = 2.0 ** -24
     weights = 2.0 ** -11 if dtype == "bfloat16" else 2.0 ** -24
     rel = weights + 2 * ((dim + 8) * eps * score + 2.0 ** -39 * spread) + 2.0 ** -20 + 2 * (64 + positions / 64) * eps
-    return torch.finfo(TORCH[dtype]).eps / 2 * np.abs(want) + rel * weight + 2.0 ** -39 * size + 1e-30
+    return torch.finfo(TORCH[dtype]).eps / 2 * np.abs(want) + rel * weight + 2.0 ** -32 * size + 1e-30
 
 
 def check(dtype, got, q, held, pos, seq, window, scale, dim, nh):
