@@ -476,87 +476,323 @@ kv4_join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ p
 }
 
 // ============================================================================ prompt portions
-__device__ inline void kv4_attend(const elem_t* q, long q_stride, const unsigned char* k_cache, const unsigned char* v_cache,
-                                  const int32_t* block_table, int table_stride, const int32_t* positions, const int32_t* seq_rows,
-                                  elem_t* out, int t, int qh, int n_heads, int n_kv_heads, int head_dim, int page_size, int window,
-                                  float scale, float* qs, float* es) {
-  const int lane = threadIdx.x, kvh = qh / (n_heads / n_kv_heads), pos = positions[t];
-  elem_t* orow = out + ((size_t)t * n_heads + qh) * head_dim;
-  if (pos < 0) {
-    for (int d = lane; d < head_dim; d += AXON_WAVE) orow[d] = from_float(0.0f);
-    return;
-  }
-  const int lo = window > 0 ? max(0, pos + 1 - window) : 0;
-  const int32_t* table_row = block_table + (size_t)seq_rows[t] * table_stride;
-  for (int d = lane; d < head_dim; d += AXON_WAVE) qs[d] = to_float(q[t * q_stride + (size_t)qh * head_dim + d]);
-  __syncthreads();
-  const size_t head_bytes = (size_t)page_size * kv4_row_bytes(head_dim);
-  float M = -INFINITY, L = 0.0f, O[2] = {0.0f, 0.0f};
-  for (int b0 = lo / 64 * 64; b0 <= pos; b0 += 64) {
-    const int p = b0 + lane;
-    const bool live = p >= lo && p <= pos;
-    float s = -INFINITY;
-    if (live) {
-      const unsigned char* base = k_cache + ((size_t)table_row[p / page_size] * n_kv_heads + kvh) * head_bytes;
-      const int slot = p % page_size;
-      float dot = 0.0f;
-      for (int w = 0; w < head_dim / 8; ++w) {
-        const unsigned word = reinterpret_cast<const unsigned*>(base)[slot * (head_dim / 8) + w];
-        const unsigned meta = reinterpret_cast<const uint16_t*>(base + page_size * head_dim / 2)[slot * (head_dim / 32) + w / 4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dot = fmaf(qs[8 * w + i], kv4_value(__builtin_rotateright32(word, kv4_place(i)) & 15u, meta), dot);
-      }
-      s = dot * scale;
-    }
-    const float mn = fmaxf(M, wave_max(s));
-    const float e = live ? expf(s - mn) : 0.0f, a = M == -INFINITY ? 0.0f : expf(M - mn);
-    L = fmaf(L, a, wave_sum(e));
-    M = mn;
-    es[lane] = e;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int d = lane + i * AXON_WAVE;
-      if (d >= head_dim) continue;
-      O[i] *= a;
-      for (int j = max(lo - b0, 0); j <= min(pos - b0, 63); ++j) {
-        const int pj = b0 + j, slot = pj % page_size;
-        const unsigned char* base = v_cache + ((size_t)table_row[pj / page_size] * n_kv_heads + kvh) * head_bytes;
-        const unsigned word = reinterpret_cast<const unsigned*>(base)[(slot / 8) * head_dim + d];
-        const unsigned meta =
-            reinterpret_cast<const uint16_t*>(base + page_size * head_dim / 2)[((slot / 8) * (head_dim / 32) + d / 32) * 8 + slot % 8];
-        O[i] = fmaf(es[j], kv4_value(__builtin_rotateright32(word, kv4_place(slot & 7)) & 15u, meta), O[i]);
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (lane + i * AXON_WAVE < head_dim) orow[lane + i * AXON_WAVE] = from_float(__fdiv_rn(O[i], L));
+// A workgroup has a tile of up to 128 consecutive tokens of one request and HPB query heads of a key head, four waves a head, 32 rows each;
+// grid (pairs of tiles, key heads x sets of HPB heads).  A block of 64 positions is unpacked once a workgroup, an octet of slots a
+// wave, into half precision in LDS, where all waves read it: K [64][HD] and V^T [HD][64], 16-byte pieces of a row permuted so that
+// sixteen neighbouring rows' pieces lie in different banks.  Two stages: block b + 1 is unpacked, and block b + 2 on its way in registers
+// (four and a half bits a number, so few), beside the products of block b.
+// S^T = K Q^T and O^T = V^T P^T by 32x32x16 products: what a lane holds of the first is its operand of the second.  Row r of a tile
+// of S^T is position pi(r) of it, pi swapping bits 2 and 3, so that register e of tile pt is position 32 pt + 16 (e / 8) + 8 half + e % 8.
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+#define KV4_ROWS 128               // tokens of a tile
+
+__device__ __forceinline__ f32x16 kv4_mma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-__global__ void __launch_bounds__(AXON_WAVE)
-kv4_attention_kernel(const elem_t* __restrict__ q, long q_stride, const unsigned char* __restrict__ k_cache,
-                     const unsigned char* __restrict__ v_cache, const int32_t* __restrict__ block_table, int table_stride,
-                     const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows, elem_t* __restrict__ out,
-                     const int32_t* __restrict__ token_index, const int32_t* __restrict__ tiles, int n_heads, int n_kv_heads,
-                     int head_dim, int page_size, int window, float scale) {
-  __shared__ float qs[128], es[AXON_WAVE];
-  int t = blockIdx.x;
-  if (tiles) {
-    const int32_t* mine = tiles + 4 * (blockIdx.x / 256) + 2 * (blockIdx.x / 128 % 2);
-    if ((int)(blockIdx.x % 128) >= mine[1]) return;
-    t = mine[0] + blockIdx.x % 128;
-  } 
-  kv4_attend(q, q_stride, k_cache, v_cache, block_table, table_stride, positions, seq_rows, out, t, blockIdx.y, n_heads, n_kv_heads,
-             head_dim, page_size, window, scale, qs, es);
+template <int HD>
+struct Kv4Stage {
+  static constexpr int K_BYTES = KV4_BLOCK * HD * 2, BYTES = 2 * K_BYTES;
+  // where the 16 bytes of dims 8 chunk .. of a row of K, of positions 8 octet .. of a dim's row of V^T lie
+  __device__ static __forceinline__ int k_at(int row, int chunk) {
+    return row * (HD * 2) + ((chunk ^ (HD == 128 ? row & 15 : (row >> 1) & 7)) << 4);
+  }
+  __device__ static __forceinline__ int v_at(int dim, int octet) { return K_BYTES + dim * 128 + ((octet ^ ((dim >> 1) & 7)) << 4); }
+};
+
+// An octet of slots of one head on its way: a lane has HD/64 words of a row of K (eight lanes a row) and of V^T (neighbouring dims).
+template <int HD>
+struct Kv4Octet {
+  unsigned k[HD / 64], v[HD / 64], k_scale;
+  uint4 v_scale;
+};
+
+template <int HD>
+__device__ __forceinline__ void kv4_load(Kv4Octet<HD>& out, const unsigned char* k_cache, const unsigned char* v_cache, int page, int p,
+                                         size_t page_bytes, size_t head_at, int page_size, int lane) {
+  const int octet = (p & (page_size - 1)) >> 3;
+  const size_t base = page * page_bytes + head_at;                 // (all of it the wave's)
+  const unsigned words = octet * (4 * HD), scales = page_size * (HD / 2) + octet * (HD / 2);
+  const unsigned char *k = k_cache + base, *v = v_cache + base;
+  if constexpr (HD == 128) {
+    const uint2 a = *reinterpret_cast<const uint2*>(k + (words + lane * 8)), b = *reinterpret_cast<const uint2*>(v + (words + lane * 8));
+    out.k[0] = a.x; out.k[1] = a.y; out.v[0] = b.x; out.v[1] = b.y;
+  } else {
+    out.k[0] = *reinterpret_cast<const unsigned*>(k + (words + lane * 4));
+    out.v[0] = *reinterpret_cast<const unsigned*>(v + (words + lane * 4));
+  }
+  // row lane / 8, group (lane % 8) / 2 of four (HD 128) or (lane % 8) / 4 of two; of V^T the group of dim HD/64 lane
+  out.k_scale = *reinterpret_cast<const uint16_t*>(k + (scales + (lane >> 3) * (HD / 16) + (lane & 7) * (HD / 64) / 4 * 2));
+  out.v_scale = *reinterpret_cast<const uint4*>(v + (scales + lane * (HD / 64) / 32 * 16));
+}
+
+// Unpacked into a stage, as octet `octet` of its block.  edge: a row of the tile sees only some of the block's positions.  Those that no row sees
+// (outside first .. last) are zeros then, and so is a value that is not a number: a row that does not see it has a weight of zero for it,
+// and zero times it has to be zero.  Where such values are is left in `nans` [group][octet], a bit a slot.
+template <int HD>
+__device__ __forceinline__ void kv4_unpack(const Kv4Octet<HD>& in, unsigned char* stage, int octet, bool edge, int p, int first, int last,
+                                           unsigned char* nans, unsigned sixteens, int lane) {
+  half2_t sc[4], cc[4];
+  kv4_pair_scale(in.k_scale | in.k_scale << 16, sc[0], cc[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) { sc[i] = sc[0]; cc[i] = cc[0]; }
+  const int row = 8 * octet + (lane >> 3);
+#pragma unroll
+  for (int w = 0; w < HD / 64; ++w)
+    *reinterpret_cast<u32x4*>(stage + Kv4Stage<HD>::k_at(row, (lane & 7) * (HD / 64) + w)) = kv4_operand(in.k[w], sc, cc, sixteens);
+  unsigned metas[4] = {in.v_scale.x, in.v_scale.y, in.v_scale.z, in.v_scale.w};
+  if (edge) {
+    unsigned mask = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned half_of = 0xffffu << (16 * (i & 1));
+      const bool nan = (metas[i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00;
+      const bool seen = p + i >= first && p + i <= last;
+      if (nan || !seen) metas[i >> 1] &= ~half_of;
+      if (nan && seen) mask |= 1u << i;
+    }
+    if (lane * (HD / 64) % 32 == 0) nans[lane * (HD / 64) / 32 * 8 + octet] = (unsigned char)mask;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) kv4_pair_scale(metas[i], sc[i], cc[i]);
+#pragma unroll
+  for (int w = 0; w < HD / 64; ++w)
+    *reinterpret_cast<u32x4*>(stage + Kv4Stage<HD>::v_at(lane * (HD / 64) + w, octet)) = kv4_operand(in.v[w], sc, cc, sixteens);
+}
+
+__device__ __forceinline__ void kv4_meet() {       // everyone's part of the stage is written, everyone has read the other
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int HD, int HPB>
+__device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, int count, const elem_t* __restrict__ q, int q_stride,
+                                                 const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
+                                                 const int32_t* __restrict__ block_table, int table_stride,
+                                                 const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows,
+                                                 elem_t* __restrict__ out, int n_heads, int n_kv_heads, int page_size, int window,
+                                                 float scale) {
+  using S = Kv4Stage<HD>;
+  constexpr int WAVES = 4 * HPB, OCTETS = 8 / WAVES, DT = HD / 32, KS = HD / 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
+  const int group = n_heads / n_kv_heads, sets = (group + HPB - 1) / HPB, kvh = blockIdx.y / sets;
+  const int in_group = (blockIdx.y % sets) * HPB + (wave >> 2), head = kvh * group + min(in_group, group - 1);
+  const int pos0 = __builtin_amdgcn_readfirstlane(positions[t0]);
+  const int my_row = (wave & 3) * 32 + l32, row = min(my_row, count - 1);
+  const bool live = in_group < group && (wave & 3) * 32 < count;             // the wave has rows of its own
+  elem_t* out_row = out + ((size_t)(t0 + row) * n_heads + head) * HD;
+  if (pos0 < 0) {                                  // padding: zeros
+    if (live && my_row < count)
+      for (int d = half * (HD / 2); d < (half + 1) * (HD / 2); ++d) out_row[d] = from_float(0.0f);
+    return;
+  }
+  const int last = pos0 + count - 1, first = window > 0 ? max(0, pos0 + 1 - window) : 0;        // what any row sees
+  const int my_pos = pos0 + row, my_lo = window > 0 ? max(0, my_pos + 1 - window) : 0;
+  const int base = first / KV4_BLOCK * KV4_BLOCK, n_blocks = (last - base) / KV4_BLOCK + 1;
+  // what all rows of the tile, of the wave, see
+  const int tile_lo = window > 0 ? max(0, last + 1 - window) : 0;
+  const int wave_hi = pos0 + (wave & 3) * 32, wave_last = min(wave_hi + 31, last), wave_lo = window > 0 ? max(0, wave_last + 1 - window) : 0;
+  const int wave_first = window > 0 ? max(0, wave_hi + 1 - window) : 0;
+
+  const int32_t* table_row = block_table + (size_t)__builtin_amdgcn_readfirstlane(seq_rows[t0]) * table_stride;
+  const size_t head_bytes = (size_t)page_size * kv4_row_bytes(HD), page_bytes = head_bytes * n_kv_heads, head_at = head_bytes * kvh;
+  const int shift = __builtin_ctz(page_size);
+  const unsigned sixteens = kv4_sixteens();
+  unsigned char* nans_of = smem + 2 * S::BYTES;
+  // an octet past the tile's last position: its page's
+  auto place = [&](int b, int n) { return min(base + b * KV4_BLOCK + 8 * (n * WAVES + wave), last); };
+  auto edge = [&](int b) { return base + b * KV4_BLOCK < tile_lo || base + b * KV4_BLOCK + KV4_BLOCK - 1 > pos0; };
+  int page[OCTETS];
+  Kv4Octet<HD> octets[OCTETS];
+  auto look_up = [&](int b) {
+#pragma unroll
+    for (int n = 0; n < OCTETS; ++n) page[n] = table_row[place(b, n) >> shift];
+  };
+  auto ask = [&](int b) {
+#pragma unroll
+    for (int n = 0; n < OCTETS; ++n) kv4_load<HD>(octets[n], k_cache, v_cache, page[n], place(b, n), page_bytes, head_at, page_size, lane);
+  };
+  auto unpack = [&](int b) {
+#pragma unroll
+    for (int n = 0; n < OCTETS; ++n)
+      kv4_unpack<HD>(octets[n], smem + (b & 1) * S::BYTES, n * WAVES + wave, edge(b), base + b * KV4_BLOCK + 8 * (n * WAVES + wave), first, last,
+                     nans_of + (b & 1) * (HD / 4), sixteens, lane);
+  };
+  look_up(0);
+  ask(0);
+  if (n_blocks > 1) look_up(1);
+
+  u32x4 qf[KS][TERMS];
+  float c;
+  {
+    const elem_t* src = q + (size_t)(t0 + row) * q_stride + (size_t)head * HD + half * 8;
+    float x[KS][8], largest = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      float a[4], b[4];
+      load4_guarded(src + ks * 16, 4, true, a);
+      load4_guarded(src + ks * 16 + 4, 4, true, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[ks][i] = a[i];
+        x[ks][4 + i] = b[i];
+        largest = fmaxf(largest, fmaxf(fabsf(a[i]), fabsf(b[i])));
+      }
+    }
+    largest = fmaxf(largest, __shfl_xor(largest, 32, AXON_WAVE));
+    const int by = kv4_query_shift(largest);
+    const float up = ldexpf(1.0f, by / 2), up2 = ldexpf(1.0f, by - by / 2);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[ks][i] = x[ks][i] * up * up2;
+      kv4_split(x[ks], qf[ks]);
+    }
+    c = ldexpf(scale * LOG2E, -by);
+  }
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+  float ref = -INFINITY, l = 0.0f;
+
+  unpack(0);
+  if (n_blocks > 1) {
+    ask(1);
+    if (n_blocks > 2) look_up(2);
+  }
+  kv4_meet();
+  const int k_row = (l32 & 0x13) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);      // pi
+  for (int b = 0; b < n_blocks; ++b) {
+    if (b + 1 < n_blocks) {
+      unpack(b + 1);
+      if (b + 2 < n_blocks) {
+        ask(b + 2);
+        if (b + 3 < n_blocks) look_up(b + 3);
+      }
+    }
+    const int p0 = base + b * KV4_BLOCK;
+    if (live && p0 <= wave_last && p0 + KV4_BLOCK - 1 >= wave_first) {
+      const unsigned char* stage = smem + (b & 1) * S::BYTES;
+      f32x16 s[2];
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[pt][e] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(stage + S::k_at(32 * pt + k_row, 2 * ks + half));
+#pragma unroll
+          for (int n = TERMS - 1; n >= 0; --n) s[pt] = kv4_mma32(a, qf[ks][n], s[pt]);
+        }
+      const bool whole = p0 + KV4_BLOCK - 1 <= wave_hi && p0 >= wave_lo;
+      if (!whole) {
+        int from = p0 + 8 * half;
+        asm volatile("" : "+v"(from));
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int p = from + 32 * pt + 16 * (e >> 3) + (e & 7);
+            s[pt][e] = p >= my_lo && p <= my_pos ? s[pt][e] : -INFINITY;
+          }
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx[pt] = fmaxf(mx[pt], s[pt][e]);
+      float top = fmaxf(mx[0], mx[1]);
+      top = fmaxf(top, __shfl_xor(top, 32, AXON_WAVE));
+      const float factor = kv4_raise(ref, __fmul_rn(top, c));
+      if (__any(factor != 1.0f)) {
+        l = __fmul_rn(l, factor);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[dt][e] = __fmul_rn(o[dt][e], factor);
+      }
+      const float add = ref == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, ref);
+      u32x4 pf[4][TERMS];
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], c, add));
+          sum[i & 1] = __fadd_rn(sum[i & 1], w[i]);
+        }
+        kv4_split(w, pf[st]);
+      }
+      l = __fadd_rn(l, __fadd_rn(sum[0], sum[1]));
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(stage + S::v_at(32 * dt + l32, 2 * st + half));
+#pragma unroll
+          for (int n = TERMS - 1; n >= 0; --n) o[dt] = kv4_mma32(a, pf[st][n], o[dt]);
+        }
+      if (edge(b)) {
+        // values that are not numbers reach the rows that see them (tile dt is a group of 32 dims)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint64_t held = *reinterpret_cast<const uint64_t*>(nans_of + (b & 1) * (HD / 4) + 8 * dt);
+          if (held == 0) continue;
+          const uint64_t low = my_lo <= p0 ? ~0ull : my_lo - p0 > 63 ? 0ull : ~0ull << (my_lo - p0), high = my_pos >= p0 + 63 ? ~0ull : ~(~0ull << max(my_pos - p0 + 1, 0));
+          if (held & low & high)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] = NAN;
+        }
+      }
+    }
+    kv4_meet();
+  }
+  if (!live || my_row >= count) return;
+  l = __fadd_rn(l, __shfl_xor(l, 32, AXON_WAVE));
+  const float inv = __fdiv_rn(1.0f, l);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      elem_t* dst = out_row + dt * 32 + g * 8 + half * 4;
+#if AXON_BF16
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2_bf16(__fmul_rn(o[dt][4 * g], inv), __fmul_rn(o[dt][4 * g + 1], inv)),
+                                                  pack2_bf16(__fmul_rn(o[dt][4 * g + 2], inv), __fmul_rn(o[dt][4 * g + 3], inv)));
+#else
+      *reinterpret_cast<float4*>(dst) = make_float4(__fmul_rn(o[dt][4 * g], inv), __fmul_rn(o[dt][4 * g + 1], inv),
+                                                    __fmul_rn(o[dt][4 * g + 2], inv), __fmul_rn(o[dt][4 * g + 3], inv));
+#endif
+    }
+}
+
+// A workgroup takes one tile or two, one after the other: tiles [n][4] = (first token, count) twice, the second count 0 if there is none.
+template <int HD, int HPB>
+__global__ void __launch_bounds__(256 * HPB, TERMS == 1 ? 2 : 1)
+kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned char* __restrict__ k_cache,
+                   const unsigned char* __restrict__ v_cache, const int32_t* __restrict__ block_table, int table_stride,
+                   const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows, elem_t* __restrict__ out,
+                   const int32_t* __restrict__ tiles, int n_heads, int n_kv_heads, int page_size, int window, float scale) {
+  extern __shared__ __align__(256) unsigned char smem[];
+  const int32_t* mine = tiles + 4 * blockIdx.x;
+  for (int part = 0; part < 2; ++part) {
+    const int t0 = mine[2 * part], count = mine[2 * part + 1];
+    if (count <= 0 || count > KV4_ROWS) break;     // the same for the whole workgroup
+    kv4_prefill_tile<HD, HPB>(smem, t0, count, q, q_stride, k_cache, v_cache, block_table, table_stride, positions, seq_rows, out, n_heads,
+                              n_kv_heads, page_size, window, scale);
+  }
 }
 
 // ============================================================================ entry points
 // Positions of a chunk of a token that sees `seen` positions.
 extern "C" int axk_kv4_decode_chunk(int seen) { return kv4_chunk(seen); }
 extern "C" int axk_kv4_decode_item_factor(void) { return KV4_ITEM_FACTOR; }
-extern "C" int axk_kv4_prefill_tile(void) { return 128; }
+extern "C" int axk_kv4_prefill_tile(void) { return KV4_ROWS; }
 
 extern "C" long axk_kv4_decode_workspace(int n_tokens, int n_heads, int head_dim, int max_chunks) {
   return (long)n_tokens * n_heads * max_chunks * (head_dim + 2);
@@ -619,11 +855,37 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
   const int rc = kv4_attention_args("kv4_attention_prefill", q, q_stride, k_cache, v_cache, out, n_heads, n_kv_heads, head_dim,
                                     page_size, window, scale);
   if (rc != 0) return rc;
-  AXK_REQUIRE(n_tiles >= 0 && n_tiles < (1 << 22), "kv4_attention_prefill: %d tiles", n_tiles);
+  AXK_REQUIRE(n_tiles >= 0 && (n_tiles == 0 || tiles != nullptr), "kv4_attention_prefill: %d tiles", n_tiles);
   if (n_tiles == 0) return 0;
-  kv4_attention_kernel<<<dim3(n_tiles * 256, n_heads), AXON_WAVE, 0, (hipStream_t)stream>>>(
-      (const elem_t*)q, q_stride, (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride, positions,
-      seq_rows, (elem_t*)out, nullptr, tiles, n_heads, n_kv_heads, head_dim, page_size, window, scale);
+  const int group = n_heads / n_kv_heads;
+#define LAUNCH(HD, HPB)                                                                                                         \
+  {                                                                                                                             \
+    constexpr int lds = 2 * Kv4Stage<HD>::BYTES + 2 * (HD / 4);                                                                 \
+    static bool configured = false;                                                                                             \
+    if (!configured) {                                                                                                          \
+      hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<HD, HPB>),                           \
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, lds);                                      \
+      if (e != hipSuccess) {                                                                                                    \
+        axk_set_error("kv4_attention_prefill: cannot reserve %d bytes of LDS: %s", lds, hipGetErrorString(e));                  \
+        return -2;                                                                                                              \
+      }                                                                                                                         \
+      configured = true;                                                                                                        \
+    }                                                                                                                           \
+    AXK_INSTANCE(INST_KV4_PREFILL, HD, HPB);                                                                                    \
+    kv4_prefill_kernel<HD, HPB><<<dim3(n_tiles, n_kv_heads * ((group + HPB - 1) / HPB)), 256 * HPB, lds, (hipStream_t)stream>>>( \
+        (const elem_t*)q, q_stride, (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride,    \
+        positions, seq_rows, (elem_t*)out, tiles, n_heads, n_kv_heads, page_size, window, scale);                               \
+  }
+#if AXON_BF16
+  // one query head a workgroup while such workgroups find a CU each; beyond that two, which share what is unpacked
+  if (group >= 2 && (long)n_tiles * n_heads > 256) {
+    if (head_dim == 64) LAUNCH(64, 2) else LAUNCH(128, 2)
+  } else
+#endif
+  {
+    if (head_dim == 64) LAUNCH(64, 1) else LAUNCH(128, 1)
+  }
+#undef LAUNCH
   AXK_LAUNCH_CHECK("kv4_attention_prefill");
   return 0;
 }
