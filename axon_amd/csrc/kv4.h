@@ -50,25 +50,27 @@ __device__ inline float kv4_scale_of(unsigned meta) {
   return (float)__builtin_bit_cast(_Float16, (unsigned short)(meta & 0x7FE0));
 }
 
+// The constants of the unpacking, in registers: as constants the compiler takes two instructions for both masks, not one.
+struct Kv4Masks {
+  unsigned digit, sixteens;
+};
+__device__ __forceinline__ Kv4Masks kv4_masks() {
+  Kv4Masks m = {0x03C003C0u, 0x4C004C00u};
+  asm("" : "+s"(m.digit));
+  asm("" : "+v"(m.sixteens));
+  return m;
+}
+
 // A word's eight numbers as an operand of the matrix cores; s and c hold the scales and -(16 + z) s of each pair.  Eleven
-// instructions for eight numbers: three rotations, four times both masks in one (with the constants in registers: left to
-// itself the compiler takes two instructions with a constant each), four packed multiply-adds.
-__device__ __forceinline__ u32x4 kv4_operand(unsigned word, const half2_t (&s)[4], const half2_t (&c)[4], unsigned sixteens) {
+// instructions for eight numbers: three rotations, four times both masks, four packed multiply-adds.
+__device__ __forceinline__ u32x4 kv4_operand(unsigned word, const half2_t (&s)[4], const half2_t (&c)[4], const Kv4Masks& masks) {
   u32x4 out;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    unsigned x = __builtin_rotateright32(word, 4 * i);
-    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(x) : "v"(x), "s"(0x03C003C0u), "v"(sixteens));
+    const unsigned x = (__builtin_rotateright32(word, 4 * i) & masks.digit) | masks.sixteens;
     out[i] = __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(half2_t, x), s[i], c[i]));
   }
   return out;
-}
-
-// The pair 16, 16 in a register.
-__device__ __forceinline__ unsigned kv4_sixteens() {
-  unsigned v = 0x4C004C00u;
-  asm("" : "+v"(v));
-  return v;
 }
 
 // The scales of two numbers, from a pair of scale words.

@@ -156,7 +156,7 @@ __device__ __forceinline__ void kv4_load(Kv4Values<HD>& out, const Kv4Place& at,
 
 // S^T of a block: s[2 u + v][r] is position 32 u + 8 h + 4 v + r of column l16, unscaled.
 template <int HD>
-__device__ __forceinline__ void kv4_scores(const Kv4Keys<HD>& keys, const u32x4 (&qf)[HD / 32][TERMS], unsigned sixteens, f32x4 (&s)[4]) {
+__device__ __forceinline__ void kv4_scores(const Kv4Keys<HD>& keys, const u32x4 (&qf)[HD / 32][TERMS], const Kv4Masks& masks, f32x4 (&s)[4]) {
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     half2_t sc[4], cc[4];
@@ -166,7 +166,7 @@ __device__ __forceinline__ void kv4_scores(const Kv4Keys<HD>& keys, const u32x4 
     s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) {
-      const u32x4 a = kv4_operand(keys.words[t][j], sc, cc, sixteens);
+      const u32x4 a = kv4_operand(keys.words[t][j], sc, cc, masks);
 #pragma unroll
       for (int n = TERMS - 1; n >= 0; --n) s[t] = kv4_mma(a, qf[j][n], s[t]);
     }
@@ -221,7 +221,7 @@ __device__ __forceinline__ void kv4_weights(f32x4 (&s)[4], bool whole, int p0, i
 // The block's values, weighted, added to the column's output: o[dt][r] is dim HD/16 (4 h + r) + dt of column l16.
 template <int HD>
 __device__ __forceinline__ void kv4_values(const Kv4Values<HD>& values, const u32x4 (&pf)[2][TERMS], bool whole, int p0, int lo, int pos,
-                                           int lane, unsigned sixteens, f32x4 (&o)[HD / 16]) {
+                                           int lane, const Kv4Masks& masks, f32x4 (&o)[HD / 16]) {
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     unsigned metas[4] = {values.scale[u].x, values.scale[u].y, values.scale[u].z, values.scale[u].w};
@@ -242,7 +242,7 @@ __device__ __forceinline__ void kv4_values(const Kv4Values<HD>& values, const u3
     for (int dt = 0; dt < HD / 16; ++dt) {
       const uint4 four = values.words[u][dt / 4];
       const unsigned word = dt % 4 == 0 ? four.x : dt % 4 == 1 ? four.y : dt % 4 == 2 ? four.z : four.w;
-      const u32x4 a = kv4_operand(word, sc, cc, sixteens);
+      const u32x4 a = kv4_operand(word, sc, cc, masks);
 #pragma unroll
       for (int n = TERMS - 1; n >= 0; --n) o[dt] = kv4_mma(a, pf[u][n], o[dt]);
       if (dt % 2) __builtin_amdgcn_sched_barrier(0);       // (else every tile is unpacked before the first product)
@@ -338,7 +338,7 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (b_first <= b_last) {
-    const unsigned sixteens = kv4_sixteens();
+    Kv4Masks masks = kv4_masks();
     Kv4Keys<HD> keys;
     Kv4Values<HD> values;
     kv4_load<HD>(keys, at, b_first, lane);
@@ -351,7 +351,7 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
       const bool whole = p0 >= lo && p0 + KV4_BLOCK - 1 <= pos;
       f32x4 s[4];
       u32x4 pf[2][TERMS];
-      kv4_scores<HD>(keys, qf, sixteens, s);
+      kv4_scores<HD>(keys, qf, masks, s);
       __builtin_amdgcn_sched_barrier(0);
       if (b < b_last) kv4_load<HD>(keys, at, b + 1, lane);
       __builtin_amdgcn_sched_barrier(0);
@@ -361,7 +361,7 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[dt][r] = __fmul_rn(o[dt][r], factor);
       });
-      kv4_values<HD>(values, pf, whole, p0, lo, pos, lane, sixteens, o);
+      kv4_values<HD>(values, pf, whole, p0, lo, pos, lane, masks, o);
       __builtin_amdgcn_sched_barrier(0);
       if (b < b_last) kv4_load<HD>(values, at, b + 1, lane);
       __builtin_amdgcn_sched_barrier(0);
@@ -492,12 +492,15 @@ __device__ __forceinline__ f32x16 kv4_mma32(u32x4 a, u32x4 b, f32x16 c) {
 
 template <int HD>
 struct Kv4Stage {
-  static constexpr int K_BYTES = KV4_BLOCK * HD * 2, BYTES = 2 * K_BYTES;
+  static constexpr int K_BYTES = KV4_BLOCK * HD * 2, BYTES = 2 * K_BYTES, ALL = 2 * BYTES + 2 * (HD / 4);
+  // a row's pieces are permuted by this
+  __device__ static __forceinline__ int k_swizzle(int row) { return HD == 128 ? row & 15 : (row >> 1) & 7; }
+  __device__ static __forceinline__ int v_swizzle(int dim) { return (dim >> 1) & 7; }
   // where the 16 bytes of dims 8 chunk .. of a row of K, of positions 8 octet .. of a dim's row of V^T lie
   __device__ static __forceinline__ int k_at(int row, int chunk) {
-    return row * (HD * 2) + ((chunk ^ (HD == 128 ? row & 15 : (row >> 1) & 7)) << 4);
+    return row * (HD * 2) + ((chunk ^ k_swizzle(row)) << 4);
   }
-  __device__ static __forceinline__ int v_at(int dim, int octet) { return K_BYTES + dim * 128 + ((octet ^ ((dim >> 1) & 7)) << 4); }
+  __device__ static __forceinline__ int v_at(int dim, int octet) { return K_BYTES + dim * 128 + ((octet ^ v_swizzle(dim)) << 4); }
 };
 
 // An octet of slots of one head on its way: a lane has HD/64 words of a row of K (eight lanes a row) and of V^T (neighbouring dims).
@@ -526,38 +529,42 @@ __device__ __forceinline__ void kv4_load(Kv4Octet<HD>& out, const unsigned char*
   out.v_scale = *reinterpret_cast<const uint4*>(v + (scales + lane * (HD / 64) / 32 * 16));
 }
 
-// Unpacked into a stage, as octet `octet` of its block.  edge: a row of the tile sees only some of the block's positions.  Those that no row sees
-// (outside first .. last) are zeros then, and so is a value that is not a number: a row that does not see it has a weight of zero for it,
-// and zero times it has to be zero.  Where such values are is left in `nans` [group][octet], a bit a slot.
+// For a block of which a row of the tile sees only some positions: the values' scales of those that no row sees (outside first .. last) become
+// zero, and so do those of values that are not numbers: a row that does not see them has a weight of zero for them, and
+// zero times them has to be zero.  Where such values are is left in `nans` [group][octet], a bit a slot.
 template <int HD>
-__device__ __forceinline__ void kv4_unpack(const Kv4Octet<HD>& in, unsigned char* stage, int octet, bool edge, int p, int first, int last,
-                                           unsigned char* nans, unsigned sixteens, int lane) {
-  half2_t sc[4], cc[4];
-  kv4_pair_scale(in.k_scale | in.k_scale << 16, sc[0], cc[0]);
+__device__ __forceinline__ void kv4_edge(Kv4Octet<HD>& in, int octet, int p, int first, int last, unsigned char* nans, int lane) {
+  unsigned metas[4] = {in.v_scale.x, in.v_scale.y, in.v_scale.z, in.v_scale.w}, mask = 0;
 #pragma unroll
-  for (int i = 1; i < 4; ++i) { sc[i] = sc[0]; cc[i] = cc[0]; }
-  const int row = 8 * octet + (lane >> 3);
-#pragma unroll
-  for (int w = 0; w < HD / 64; ++w)
-    *reinterpret_cast<u32x4*>(stage + Kv4Stage<HD>::k_at(row, (lane & 7) * (HD / 64) + w)) = kv4_operand(in.k[w], sc, cc, sixteens);
-  unsigned metas[4] = {in.v_scale.x, in.v_scale.y, in.v_scale.z, in.v_scale.w};
-  if (edge) {
-    unsigned mask = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned half_of = 0xffffu << (16 * (i & 1));
-      const bool nan = (metas[i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00;
-      const bool seen = p + i >= first && p + i <= last;
-      if (nan || !seen) metas[i >> 1] &= ~half_of;
-      if (nan && seen) mask |= 1u << i;
-    }
-    if (lane * (HD / 64) % 32 == 0) nans[lane * (HD / 64) / 32 * 8 + octet] = (unsigned char)mask;
+  for (int i = 0; i < 8; ++i) {
+    const bool nan = (metas[i >> 1] >> (16 * (i & 1)) & 0x7C00) == 0x7C00;
+    const bool seen = p + i >= first && p + i <= last;
+    if (nan || !seen) metas[i >> 1] &= ~(0xffffu << (16 * (i & 1)));
+    if (nan && seen) mask |= 1u << i;
   }
+  if (lane * (HD / 64) % 32 == 0) nans[lane * (HD / 64) / 32 * 8 + octet] = (unsigned char)mask;
+  in.v_scale = make_uint4(metas[0], metas[1], metas[2], metas[3]);
+}
+
+// Unpacked into a stage, as octet `octet` of its block, in PIECES pieces (0, 1: keys, 2, 3: values).
+#define KV4_PIECES 4
+template <int HD>
+__device__ __forceinline__ void kv4_unpack(const Kv4Octet<HD>& in, unsigned char* stage, int octet, int piece, const Kv4Masks& masks, int lane) {
+  half2_t sc[4], cc[4];
+  const int w = piece & 1;
+  if (w >= HD / 64) return;
+  if (piece < 2) {
+    kv4_pair_scale(in.k_scale | in.k_scale << 16, sc[0], cc[0]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) kv4_pair_scale(metas[i], sc[i], cc[i]);
+    for (int i = 1; i < 4; ++i) { sc[i] = sc[0]; cc[i] = cc[0]; }
+    *reinterpret_cast<u32x4*>(stage + Kv4Stage<HD>::k_at(8 * octet + (lane >> 3), (lane & 7) * (HD / 64) + w)) =
+        kv4_operand(in.k[w], sc, cc, masks);
+  } else {
+    const unsigned metas[4] = {in.v_scale.x, in.v_scale.y, in.v_scale.z, in.v_scale.w};
 #pragma unroll
-  for (int w = 0; w < HD / 64; ++w)
-    *reinterpret_cast<u32x4*>(stage + Kv4Stage<HD>::v_at(lane * (HD / 64) + w, octet)) = kv4_operand(in.v[w], sc, cc, sixteens);
+    for (int i = 0; i < 4; ++i) kv4_pair_scale(metas[i], sc[i], cc[i]);
+    *reinterpret_cast<u32x4*>(stage + Kv4Stage<HD>::v_at(lane * (HD / 64) + w, octet)) = kv4_operand(in.v[w], sc, cc, masks);
+  }
 }
 
 __device__ __forceinline__ void kv4_meet() {       // everyone's part of the stage is written, everyone has read the other
@@ -598,7 +605,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   const int32_t* table_row = block_table + (size_t)__builtin_amdgcn_readfirstlane(seq_rows[t0]) * table_stride;
   const size_t head_bytes = (size_t)page_size * kv4_row_bytes(HD), page_bytes = head_bytes * n_kv_heads, head_at = head_bytes * kvh;
   const int shift = __builtin_ctz(page_size);
-  const unsigned sixteens = kv4_sixteens();
+  Kv4Masks masks = kv4_masks();
   unsigned char* nans_of = smem + 2 * S::BYTES;
   // an octet past the tile's last position: its page's
   auto place = [&](int b, int n) { return min(base + b * KV4_BLOCK + 8 * (n * WAVES + wave), last); };
@@ -613,15 +620,23 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
 #pragma unroll
     for (int n = 0; n < OCTETS; ++n) kv4_load<HD>(octets[n], k_cache, v_cache, page[n], place(b, n), page_bytes, head_at, page_size, lane);
   };
-  auto unpack = [&](int b) {
+  auto mend = [&](int b) {
+    if (edge(b))
 #pragma unroll
-    for (int n = 0; n < OCTETS; ++n)
-      kv4_unpack<HD>(octets[n], smem + (b & 1) * S::BYTES, n * WAVES + wave, edge(b), base + b * KV4_BLOCK + 8 * (n * WAVES + wave), first, last,
-                     nans_of + (b & 1) * (HD / 4), sixteens, lane);
+      for (int n = 0; n < OCTETS; ++n)
+        kv4_edge<HD>(octets[n], n * WAVES + wave, base + b * KV4_BLOCK + 8 * (n * WAVES + wave), first, last, nans_of + (b & 1) * (HD / 4), lane);
+  };
+  auto unpack = [&](int b, int piece) {
+#pragma unroll
+    for (int n = 0; n < OCTETS; ++n) kv4_unpack<HD>(octets[n], smem + (b & 1) * S::BYTES, n * WAVES + wave, piece, masks, lane);
+  };
+  auto unpack_all = [&](int b) {
+#pragma unroll
+    for (int piece = 0; piece < KV4_PIECES; ++piece) unpack(b, piece);
   };
   look_up(0);
   ask(0);
-  if (n_blocks > 1) look_up(1);
+  look_up(1);
 
   u32x4 qf[KS][TERMS];
   float c;
@@ -658,37 +673,72 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
   float ref = -INFINITY, l = 0.0f;
 
-  unpack(0);
-  if (n_blocks > 1) {
-    ask(1);
-    if (n_blocks > 2) look_up(2);
-  }
+  // (what is asked for past the last block is of the last page, and is not used)
+  mend(0);
+  unpack_all(0);
+  ask(1);
+  look_up(2);
   kv4_meet();
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) void*)smem;
   const int k_row = (l32 & 0x13) | ((l32 & 4) << 1) | ((l32 & 8) >> 1);      // pi
-  for (int b = 0; b < n_blocks; ++b) {
-    if (b + 1 < n_blocks) {
-      unpack(b + 1);
-      if (b + 2 < n_blocks) {
-        ask(b + 2);
-        if (b + 3 < n_blocks) look_up(b + 3);
-      }
-    }
+  // the wave's part of a block that none of its rows sees
+  auto pass = [&](int b) {
+    mend(b + 1);
+    unpack_all(b + 1);
+    ask(b + 2);
+    look_up(b + 3);
+    kv4_meet();
+  };
+  const int from = live ? max(0, wave_first - base) / KV4_BLOCK : n_blocks, to = live ? (wave_last - base) / KV4_BLOCK : -1;
+  unsigned nan_groups = 0;                         // groups of 32 dims in which the lane's row sees a value that is not a number
+  int b = 0;
+  for (; b < from; ++b) pass(b);
+  for (; b <= to; ++b) {
     const int p0 = base + b * KV4_BLOCK;
-    if (live && p0 <= wave_last && p0 + KV4_BLOCK - 1 >= wave_first) {
-      const unsigned char* stage = smem + (b & 1) * S::BYTES;
+    mend(b + 1);
+    {
+      // A row begins at a multiple of its size, and piece 2 n + half of it is piece `half` with n's bits exclusive-ored in: one instruction from a
+      // base each.  The bases are opaque, or the compiler keeps every address in a register across the loop.
+      unsigned k_base = lds0 + (b & 1) * S::BYTES + k_row * (HD * 2) + ((half ^ S::k_swizzle(k_row)) << 4);
+      unsigned v_base = lds0 + (b & 1) * S::BYTES + S::K_BYTES + l32 * 128 + ((half ^ S::v_swizzle(l32)) << 4);
+      asm volatile("" : "+v"(k_base), "+v"(v_base));
+      // The scores, fragments read two groups of products ahead, and the next block unpacked a piece behind each group: the matrix cores
+      // work on the group meanwhile.
+      constexpr int GROUPS = KS / 2;
       f32x16 s[2];
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[pt][e] = 0.0f;
+      u32x4 kf[3][4];
+      auto read_k = [&](int g) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int pt = 0; pt < 2; ++pt) {
-          const u32x4 a = *reinterpret_cast<const u32x4*>(stage + S::k_at(32 * pt + k_row, 2 * ks + half));
-#pragma unroll
-          for (int n = TERMS - 1; n >= 0; --n) s[pt] = kv4_mma32(a, qf[ks][n], s[pt]);
+        for (int kk = 0; kk < 2; ++kk) {
+          const unsigned at = k_base ^ ((2 * g + kk) << 5);
+          lds_read16<0>(kf[g % 3][2 * kk], at);
+          lds_read16<32 * HD * 2>(kf[g % 3][2 * kk + 1], at);
         }
+      };
+      read_k(0);
+      read_k(1);
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        if (g + 2 < GROUPS) read_k(g + 2);
+        if (g + 2 < GROUPS) wait_lgkmcnt<8>();
+        else if (g + 1 < GROUPS) wait_lgkmcnt<4>();
+        else wait_lgkmcnt<0>();
+        use_frags<4>(kf[g % 3]);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int n = TERMS - 1; n >= 0; --n)
+#pragma unroll
+            for (int pt = 0; pt < 2; ++pt) s[pt] = kv4_mma32(kf[g % 3][2 * kk + pt], qf[2 * g + kk][n], s[pt]);
+#pragma unroll
+        for (int piece = 0; piece < KV4_PIECES / GROUPS; ++piece) unpack(b + 1, g * (KV4_PIECES / GROUPS) + piece);
+      }
+      ask(b + 2);
+      look_up(b + 3);
       const bool whole = p0 + KV4_BLOCK - 1 <= wave_hi && p0 >= wave_lo;
       if (!whole) {
         int from = p0 + 8 * half;
@@ -717,47 +767,52 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
           for (int e = 0; e < 16; ++e) o[dt][e] = __fmul_rn(o[dt][e], factor);
       }
       const float add = ref == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, ref);
-      u32x4 pf[4][TERMS];
+      // The weights of sixteen positions, then their products with all dims: on those the matrix cores work while the vector unit has the weights
+      // of the next sixteen.
       float sum[2] = {0.0f, 0.0f};
+      u32x4 vf[2][DT];
+      auto read_v = [&](int st) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) lds_read16_step<32 * 128, DT>(vf[st & 1][dt], v_base ^ (st << 5), dt);
+      };
+      read_v(0);
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
+        if (st + 1 < 4) read_v(st + 1);
         float w[8];
+        u32x4 pf[TERMS];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], c, add));
           sum[i & 1] = __fadd_rn(sum[i & 1], w[i]);
         }
-        kv4_split(w, pf[st]);
+        kv4_split(w, pf);
+        if (st + 1 < 4) wait_lgkmcnt<DT>();
+        else wait_lgkmcnt<0>();
+        use_frags<DT>(vf[st & 1]);
+#pragma unroll
+        for (int n = TERMS - 1; n >= 0; --n)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt] = kv4_mma32(vf[st & 1][dt], pf[n], o[dt]);
       }
       l = __fadd_rn(l, __fadd_rn(sum[0], sum[1]));
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          const u32x4 a = *reinterpret_cast<const u32x4*>(stage + S::v_at(32 * dt + l32, 2 * st + half));
-#pragma unroll
-          for (int n = TERMS - 1; n >= 0; --n) o[dt] = kv4_mma32(a, pf[st][n], o[dt]);
-        }
       if (edge(b)) {
-        // values that are not numbers reach the rows that see them (tile dt is a group of 32 dims)
+        const uint64_t low = my_lo <= p0 ? ~0ull : my_lo - p0 > 63 ? 0ull : ~0ull << (my_lo - p0),
+                       high = my_pos >= p0 + 63 ? ~0ull : ~(~0ull << max(my_pos - p0 + 1, 0));
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const uint64_t held = *reinterpret_cast<const uint64_t*>(nans_of + (b & 1) * (HD / 4) + 8 * dt);
-          if (held == 0) continue;
-          const uint64_t low = my_lo <= p0 ? ~0ull : my_lo - p0 > 63 ? 0ull : ~0ull << (my_lo - p0), high = my_pos >= p0 + 63 ? ~0ull : ~(~0ull << max(my_pos - p0 + 1, 0));
-          if (held & low & high)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[dt][e] = NAN;
-        }
+        for (int dt = 0; dt < DT; ++dt)
+          if (*reinterpret_cast<const uint64_t*>(nans_of + (b & 1) * (HD / 4) + 8 * dt) & low & high) nan_groups |= 1u << dt;
       }
     }
     kv4_meet();
   }
+  for (; b < n_blocks; ++b) pass(b);
   if (!live || my_row >= count) return;
   l = __fadd_rn(l, __shfl_xor(l, 32, AXON_WAVE));
-  const float inv = __fdiv_rn(1.0f, l);
+  const float all = __fdiv_rn(1.0f, l);
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+  for (int dt = 0; dt < DT; ++dt) {
+    const float inv = nan_groups >> dt & 1 ? NAN : all;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       elem_t* dst = out_row + dt * 32 + g * 8 + half * 4;
@@ -769,6 +824,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
                                                     __fmul_rn(o[dt][4 * g + 2], inv), __fmul_rn(o[dt][4 * g + 3], inv));
 #endif
     }
+  }
 }
 
 // A workgroup takes one tile or two, one after the other: tiles [n][4] = (first token, count) twice, the second count 0 if there is none.
@@ -860,7 +916,7 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
   const int group = n_heads / n_kv_heads;
 #define LAUNCH(HD, HPB)                                                                                                         \
   {                                                                                                                             \
-    constexpr int lds = 2 * Kv4Stage<HD>::BYTES + 2 * (HD / 4);                                                                 \
+    constexpr int lds = Kv4Stage<HD>::ALL;                                                                 \
     static bool configured = false;                                                                                             \
     if (!configured) {                                                                                                          \
       hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<HD, HPB>),                           \
