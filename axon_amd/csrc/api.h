@@ -525,7 +525,7 @@ int axk_rope_kv4_write(const void* qkv, long qkv_stride, void* q_out, long q_str
 int axk_kv4_read(const void* k_cache, const void* v_cache, const int32_t* block_table, int table_stride, const int32_t* positions,
                  const int32_t* seq_rows, void* k_out, void* v_out, int n_rows, int n_kv_heads, int head_dim, int page_size,
                  void* stream);
-// Causal attention over it; arguments, work lists and tiles as axk_attention_decode and axk_attention_prefill take them.
+// Causal attention over it; arguments as axk_attention_decode and axk_attention_prefill take them, but for the work lists and tiles.
 // A token that sees `seen` positions is cut into chunks of axk_kv4_decode_chunk(seen) positions, at multiples of that.
 int axk_kv4_decode_chunk(int seen);
 int axk_kv4_decode_item_factor(void);
@@ -535,11 +535,17 @@ int axk_kv4_attention_decode(const void* q, int q_stride, const void* k_cache, c
                              const int32_t* token_index, int n_tokens, const int32_t* work, int n_work, float* partial,
                              int max_chunks, int n_heads, int n_kv_heads, int head_dim, int page_size, int window, float scale,
                              void* stream);
+// Prompt portions: tiles [n_tiles][4] = (first token, count up to axk_kv4_prefill_tile, segment, slot).  segment -1: everything that the
+// tile's rows see, which needs a slot of the workspace (its own, else -1) if that reaches over a multiple of axk_kv4_prefill_segment positions;
+// segment s: only positions s x axk_kv4_prefill_segment and up to the next, into its slot; segment -1 - n: the tile's n segments, which lie in
+// n slots from `slot` on, are folded into its rows of out (by a second launch).  The same bits either way.
 int axk_kv4_prefill_tile(void);
+int axk_kv4_prefill_segment(void);
+long axk_kv4_prefill_workspace(int n_slots, int n_heads, int head_dim);
 int axk_kv4_attention_prefill(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int32_t* block_table,
                               int table_stride, const int32_t* positions, const int32_t* seq_rows, void* out, const int32_t* tiles,
-                              int n_tiles, int n_heads, int n_kv_heads, int head_dim, int page_size, int window, float scale,
-                              void* stream);
+                              int n_tiles, float* partial, long partial_floats, int n_heads, int n_kv_heads, int head_dim, int page_size,
+                              int window, float scale, void* stream);
 
 #ifdef __cplusplus
 }

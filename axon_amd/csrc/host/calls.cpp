@@ -31,7 +31,8 @@
   X(axk_masked_attention) X(axk_concat_round) X(axk_fill_i32) X(axk_fill_f32) X(axk_attention_decode_workspace) \
   X(axk_gemm_workspace) X(axk_argmax_workspace) X(axk_latent_attention_workspace) X(axk_masked_attention_workspace) \
   X(axk_delta_chunked_workspace) X(axk_kv4_ok) X(axk_kv4_row_bytes) X(axk_rope_kv4_write) X(axk_kv4_read) \
-  X(axk_kv4_decode_workspace) X(axk_kv4_attention_decode) X(axk_kv4_attention_prefill)
+  X(axk_kv4_decode_workspace) X(axk_kv4_attention_decode) \
+  X(axk_kv4_prefill_workspace) X(axk_kv4_attention_prefill)
 
 namespace {
 

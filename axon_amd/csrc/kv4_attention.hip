@@ -477,7 +477,7 @@ kv4_join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ p
 
 // ============================================================================ prompt portions
 // A workgroup has a tile of up to 128 consecutive tokens of one request and HPB query heads of a key head, four waves a head, 32 rows each;
-// grid (pairs of tiles, key heads x sets of HPB heads).  A block of 64 positions is unpacked once a workgroup, an octet of slots a
+// grid (key heads x sets of HPB heads, tiles), tiles with the most work first, so that the shortest are left for the end.  A block of 64 positions is unpacked once a workgroup, an octet of slots a
 // wave, into half precision in LDS, where all waves read it: K [64][HD] and V^T [HD][64], 16-byte pieces of a row permuted so that
 // sixteen neighbouring rows' pieces lie in different banks.  Two stages: block b + 1 is unpacked, and block b + 2 on its way in registers
 // (four and a half bits a number, so few), beside the products of block b.
@@ -485,6 +485,10 @@ kv4_join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ p
 // of S^T is position pi(r) of it, pi swapping bits 2 and 3, so that register e of tile pt is position 32 pt + 16 (e / 8) + 8 half + e % 8.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 #define KV4_ROWS 128               // tokens of a tile
+// What a row sums is closed at every KV4_SEGMENT-th position and folded, in order, into what the segments before gave, whether one workgroup
+// takes them all (its sums then wait in the workspace: 2.5 % of its time) or one each, which kv4_fold_kernel joins: the
+// same bits, so a row's result does not depend on how many tiles a step has.
+#define KV4_SEGMENT 2048
 
 __device__ __forceinline__ f32x16 kv4_mma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -573,18 +577,83 @@ __device__ __forceinline__ void kv4_meet() {       // everyone's part of the sta
   asm volatile("" ::: "memory");
 }
 
+// A wave's state of a segment: its rows' outputs, references and (each half of the wave its own) sums.  Kept as the lanes hold it.
+template <int HD>
+struct Kv4State {
+  f32x16 o[HD / 32];
+  float ref, l;
+  static constexpr int FLOATS = KV4_ROWS * HD + 2 * 256;              // of a tile and head
+};
+
+template <int HD>
+__device__ __forceinline__ void kv4_store(const Kv4State<HD>& st, float* at, int wave, int lane, unsigned nan_groups) {
+#pragma unroll
+  for (int dt = 0; dt < HD / 32; ++dt) {
+    const bool nan = nan_groups >> dt & 1;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(at + (((wave * (HD / 32) + dt) * 4 + g) * 64 + lane) * 4) =
+          nan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(st.o[dt][4 * g], st.o[dt][4 * g + 1], st.o[dt][4 * g + 2], st.o[dt][4 * g + 3]);
+  }
+  *reinterpret_cast<float2*>(at + KV4_ROWS * HD + (wave * 64 + lane) * 2) = make_float2(st.ref, st.l);
+}
+
+// Two states in order, one in the lanes (LATER: the second), one in memory, into the lanes.
+template <int HD, bool LATER>
+__device__ __forceinline__ void kv4_fold(Kv4State<HD>& st, const float* at, int wave, int lane) {
+  const float2 other = *reinterpret_cast<const float2*>(at + KV4_ROWS * HD + (wave * 64 + lane) * 2);
+  const float top = fmaxf(other.x, st.ref), base = top == -INFINITY ? 0.0f : top;
+  const float f_other = __builtin_amdgcn_exp2f(__fsub_rn(other.x, base)), f_mine = __builtin_amdgcn_exp2f(__fsub_rn(st.ref, base));
+  auto join = [&](float mine, float theirs) {
+    return LATER ? __builtin_fmaf(theirs, f_other, __fmul_rn(mine, f_mine)) : __builtin_fmaf(mine, f_mine, __fmul_rn(theirs, f_other));
+  };
+#pragma unroll
+  for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 v = *reinterpret_cast<const float4*>(at + (((wave * (HD / 32) + dt) * 4 + g) * 64 + lane) * 4);
+      st.o[dt][4 * g] = join(st.o[dt][4 * g], v.x);
+      st.o[dt][4 * g + 1] = join(st.o[dt][4 * g + 1], v.y);
+      st.o[dt][4 * g + 2] = join(st.o[dt][4 * g + 2], v.z);
+      st.o[dt][4 * g + 3] = join(st.o[dt][4 * g + 3], v.w);
+    }
+  st.l = join(st.l, other.y);
+  st.ref = top;
+}
+
+template <int HD>
+__device__ __forceinline__ void kv4_store_row(const Kv4State<HD>& st, elem_t* out_row, int lane, unsigned nan_groups) {
+  const float all = __fdiv_rn(1.0f, __fadd_rn(st.l, __shfl_xor(st.l, 32, AXON_WAVE)));
+#pragma unroll
+  for (int dt = 0; dt < HD / 32; ++dt) {
+    const float inv = nan_groups >> dt & 1 ? NAN : all;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      elem_t* dst = out_row + dt * 32 + g * 8 + (lane >> 5) * 4;
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(st.o[dt][4 * g + e], inv);
+#if AXON_BF16
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+#else
+      *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+#endif
+    }
+  }
+}
+
 template <int HD, int HPB>
 __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, int count, const elem_t* __restrict__ q, int q_stride,
                                                  const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
                                                  const int32_t* __restrict__ block_table, int table_stride,
                                                  const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows,
-                                                 elem_t* __restrict__ out, int n_heads, int n_kv_heads, int page_size, int window,
-                                                 float scale) {
+                                                 elem_t* __restrict__ out, int segment, int slot, float* __restrict__ partial, int n_slots,
+                                                 int n_heads, int n_kv_heads, int page_size, int window, float scale) {
   using S = Kv4Stage<HD>;
   constexpr int WAVES = 4 * HPB, OCTETS = 8 / WAVES, DT = HD / 32, KS = HD / 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
-  const int group = n_heads / n_kv_heads, sets = (group + HPB - 1) / HPB, kvh = blockIdx.y / sets;
-  const int in_group = (blockIdx.y % sets) * HPB + (wave >> 2), head = kvh * group + min(in_group, group - 1);
+  const int group = n_heads / n_kv_heads, sets = (group + HPB - 1) / HPB, kvh = blockIdx.x / sets;
+  const int in_group = (blockIdx.x % sets) * HPB + (wave >> 2), head = kvh * group + min(in_group, group - 1);
   const int pos0 = __builtin_amdgcn_readfirstlane(positions[t0]);
   const int my_row = (wave & 3) * 32 + l32, row = min(my_row, count - 1);
   const bool live = in_group < group && (wave & 3) * 32 < count;             // the wave has rows of its own
@@ -596,7 +665,12 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   }
   const int last = pos0 + count - 1, first = window > 0 ? max(0, pos0 + 1 - window) : 0;        // what any row sees
   const int my_pos = pos0 + row, my_lo = window > 0 ? max(0, my_pos + 1 - window) : 0;
-  const int base = first / KV4_BLOCK * KV4_BLOCK, n_blocks = (last - base) / KV4_BLOCK + 1;
+  const int seg_first = first / KV4_SEGMENT, seg_last = last / KV4_SEGMENT;
+  if (segment >= 0 && (segment < seg_first || segment > seg_last)) return;
+  if ((segment >= 0 || seg_first < seg_last) && (slot < 0 || slot >= n_slots)) return;        // (no room for what has to be kept)
+  float* state_at = partial + ((size_t)max(slot, 0) * n_heads + head) * Kv4State<HD>::FLOATS;
+  const int base = max(first, segment * KV4_SEGMENT) / KV4_BLOCK * KV4_BLOCK;
+  const int end = segment >= 0 ? min(last, segment * KV4_SEGMENT + KV4_SEGMENT - 1) : last, n_blocks = (end - base) / KV4_BLOCK + 1;
   // what all rows of the tile, of the wave, see
   const int tile_lo = window > 0 ? max(0, last + 1 - window) : 0;
   const int wave_hi = pos0 + (wave & 3) * 32, wave_last = min(wave_hi + 31, last), wave_lo = window > 0 ? max(0, wave_last + 1 - window) : 0;
@@ -666,12 +740,17 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     }
     c = ldexpf(scale * LOG2E, -by);
   }
-  f32x16 o[DT];
+  Kv4State<HD> st;
+  f32x16(&o)[DT] = st.o;
+  float &ref = st.ref, &l = st.l;
+  auto clear = [&]() {
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-  float ref = -INFINITY, l = 0.0f;
+      for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+    ref = -INFINITY;
+    l = 0.0f;
+  };
 
   // (what is asked for past the last block is of the last page, and is not used)
   mend(0);
@@ -689,11 +768,14 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     look_up(b + 3);
     kv4_meet();
   };
-  const int from = live ? max(0, wave_first - base) / KV4_BLOCK : n_blocks, to = live ? (wave_last - base) / KV4_BLOCK : -1;
+  const int from = live ? max(0, wave_first - base) / KV4_BLOCK : n_blocks, to = live ? min((wave_last - base) / KV4_BLOCK, n_blocks - 1) : -1;
   unsigned nan_groups = 0;                         // groups of 32 dims in which the lane's row sees a value that is not a number
-  int b = 0;
-  for (; b < from; ++b) pass(b);
-  for (; b <= to; ++b) {
+  bool kept = false;                               // segments before this one wait in the workspace
+  for (int b = 0, seg_end; b < n_blocks; b = seg_end) {
+  seg_end = min(n_blocks, ((base + b * KV4_BLOCK) / KV4_SEGMENT + 1) * (KV4_SEGMENT / KV4_BLOCK) - base / KV4_BLOCK);
+  clear();
+  for (; b < min(from, seg_end); ++b) pass(b);
+  for (; b <= min(to, seg_end - 1); ++b) {
     const int p0 = base + b * KV4_BLOCK;
     mend(b + 1);
     {
@@ -806,42 +888,59 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     }
     kv4_meet();
   }
-  for (; b < n_blocks; ++b) pass(b);
-  if (!live || my_row >= count) return;
-  l = __fadd_rn(l, __shfl_xor(l, 32, AXON_WAVE));
-  const float all = __fdiv_rn(1.0f, l);
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    const float inv = nan_groups >> dt & 1 ? NAN : all;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      elem_t* dst = out_row + dt * 32 + g * 8 + half * 4;
-#if AXON_BF16
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2_bf16(__fmul_rn(o[dt][4 * g], inv), __fmul_rn(o[dt][4 * g + 1], inv)),
-                                                  pack2_bf16(__fmul_rn(o[dt][4 * g + 2], inv), __fmul_rn(o[dt][4 * g + 3], inv)));
-#else
-      *reinterpret_cast<float4*>(dst) = make_float4(__fmul_rn(o[dt][4 * g], inv), __fmul_rn(o[dt][4 * g + 1], inv),
-                                                    __fmul_rn(o[dt][4 * g + 2], inv), __fmul_rn(o[dt][4 * g + 3], inv));
-#endif
-    }
+  for (; b < seg_end; ++b) pass(b);
+  if (!live || (segment < 0 && seg_first == seg_last)) continue;
+  if (kept) kv4_fold<HD, true>(st, state_at, wave & 3, lane);
+  if (seg_end < n_blocks || segment >= 0) {
+    kv4_store<HD>(st, state_at, wave & 3, lane, nan_groups);
+    nan_groups = 0;
+    kept = true;
   }
+  }
+  if (!live || my_row >= count || segment >= 0) return;
+  kv4_store_row<HD>(st, out_row, lane, nan_groups);
 }
 
-// A workgroup takes one tile or two, one after the other: tiles [n][4] = (first token, count) twice, the second count 0 if there is none.
+// tiles [n][4] = (first token, count, segment or -1 for all that the tile sees, slot of the workspace); a segment below -1 is kv4_fold_kernel's.
 template <int HD, int HPB>
 __global__ void __launch_bounds__(256 * HPB, TERMS == 1 ? 2 : 1)
 kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned char* __restrict__ k_cache,
                    const unsigned char* __restrict__ v_cache, const int32_t* __restrict__ block_table, int table_stride,
                    const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows, elem_t* __restrict__ out,
-                   const int32_t* __restrict__ tiles, int n_heads, int n_kv_heads, int page_size, int window, float scale) {
+                   const int32_t* __restrict__ tiles, float* __restrict__ partial, int n_slots, int n_heads, int n_kv_heads, int page_size,
+                   int window, float scale) {
   extern __shared__ __align__(256) unsigned char smem[];
-  const int32_t* mine = tiles + 4 * blockIdx.x;
-  for (int part = 0; part < 2; ++part) {
-    const int t0 = mine[2 * part], count = mine[2 * part + 1];
-    if (count <= 0 || count > KV4_ROWS) break;     // the same for the whole workgroup
-    kv4_prefill_tile<HD, HPB>(smem, t0, count, q, q_stride, k_cache, v_cache, block_table, table_stride, positions, seq_rows, out, n_heads,
-                              n_kv_heads, page_size, window, scale);
-  }
+  const int32_t* mine = tiles + 4 * blockIdx.y;
+  const int t0 = mine[0], count = mine[1], segment = mine[2], slot = mine[3];
+  if (count <= 0 || count > KV4_ROWS || segment < -1) return;
+  kv4_prefill_tile<HD, HPB>(smem, t0, count, q, q_stride, k_cache, v_cache, block_table, table_stride, positions, seq_rows, out, segment, slot,
+                            partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);
+}
+
+// The segments of the tiles whose segments had a workgroup each, folded in order: rows (first token, count, -1 - segments, first slot).
+template <int HD>
+__global__ void __launch_bounds__(256)
+kv4_fold_kernel(elem_t* __restrict__ out, const int32_t* __restrict__ tiles, const float* __restrict__ partial, int n_slots, int n_heads) {
+  const int32_t* mine = tiles + 4 * blockIdx.y;
+  const int t0 = mine[0], count = mine[1], segments = -1 - mine[2], slot = mine[3];
+  if (count <= 0 || count > KV4_ROWS || segments < 1 || slot < 0 || slot > n_slots - segments) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x, my_row = wave * 32 + (lane & 31);
+  if (wave * 32 >= count) return;
+  const size_t tile = (size_t)n_heads * Kv4State<HD>::FLOATS;
+  const float* at = partial + slot * tile + (size_t)head * Kv4State<HD>::FLOATS;
+  Kv4State<HD> st;
+#pragma unroll
+  for (int dt = 0; dt < HD / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 v = *reinterpret_cast<const float4*>(at + (((wave * (HD / 32) + dt) * 4 + g) * 64 + lane) * 4);
+      st.o[dt][4 * g] = v.x; st.o[dt][4 * g + 1] = v.y; st.o[dt][4 * g + 2] = v.z; st.o[dt][4 * g + 3] = v.w;
+    }
+  const float2 own = *reinterpret_cast<const float2*>(at + KV4_ROWS * HD + (wave * 64 + lane) * 2);
+  st.ref = own.x;
+  st.l = own.y;
+  for (int s = 1; s < segments; ++s) kv4_fold<HD, false>(st, at + s * tile, wave, lane);
+  if (my_row < count) kv4_store_row<HD>(st, out + ((size_t)(t0 + my_row) * n_heads + head) * HD, lane, 0);
 }
 
 // ============================================================================ entry points
@@ -904,19 +1003,31 @@ extern "C" int axk_kv4_attention_decode(const void* q, int q_stride, const void*
   return 0;
 }
 
+extern "C" int axk_kv4_prefill_segment(void) { return KV4_SEGMENT; }
+
+// Floats that a slot of the tiles' workspace has.
+extern "C" long axk_kv4_prefill_workspace(int n_slots, int n_heads, int head_dim) {
+  return (long)n_slots * n_heads * (head_dim == 64 ? Kv4State<64>::FLOATS : Kv4State<128>::FLOATS);
+}
+
 extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void* k_cache, const void* v_cache,
                                          const int32_t* block_table, int table_stride, const int32_t* positions,
-                                         const int32_t* seq_rows, void* out, const int32_t* tiles, int n_tiles, int n_heads,
-                                         int n_kv_heads, int head_dim, int page_size, int window, float scale, void* stream) {
+                                         const int32_t* seq_rows, void* out, const int32_t* tiles, int n_tiles, float* partial,
+                                         long partial_floats, int n_heads, int n_kv_heads, int head_dim, int page_size, int window,
+                                         float scale, void* stream) {
   const int rc = kv4_attention_args("kv4_attention_prefill", q, q_stride, k_cache, v_cache, out, n_heads, n_kv_heads, head_dim,
                                     page_size, window, scale);
   if (rc != 0) return rc;
-  AXK_REQUIRE(n_tiles >= 0 && (n_tiles == 0 || tiles != nullptr), "kv4_attention_prefill: %d tiles", n_tiles);
+  AXK_REQUIRE(n_tiles >= 0 && n_tiles <= 65535 && (n_tiles == 0 || tiles != nullptr), "kv4_attention_prefill: %d tiles (at most 65535)", n_tiles);
+  AXK_REQUIRE(partial_floats >= 0 && (uintptr_t)partial % 16 == 0 && (partial_floats == 0 || partial != nullptr),
+              "kv4_attention_prefill: a workspace of %ld floats, 16-byte aligned", partial_floats);
   if (n_tiles == 0) return 0;
   const int group = n_heads / n_kv_heads;
+  const long slots = partial_floats / axk_kv4_prefill_workspace(1, n_heads, head_dim);
+  const int n_slots = (int)(slots < 1 << 30 ? slots : 1 << 30);
 #define LAUNCH(HD, HPB)                                                                                                         \
   {                                                                                                                             \
-    constexpr int lds = Kv4Stage<HD>::ALL;                                                                 \
+    constexpr int lds = Kv4Stage<HD>::ALL;                                                                                      \
     static bool configured = false;                                                                                             \
     if (!configured) {                                                                                                          \
       hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<HD, HPB>),                           \
@@ -928,13 +1039,13 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
       configured = true;                                                                                                        \
     }                                                                                                                           \
     AXK_INSTANCE(INST_KV4_PREFILL, HD, HPB);                                                                                    \
-    kv4_prefill_kernel<HD, HPB><<<dim3(n_tiles, n_kv_heads * ((group + HPB - 1) / HPB)), 256 * HPB, lds, (hipStream_t)stream>>>( \
+    kv4_prefill_kernel<HD, HPB><<<dim3(n_kv_heads * ((group + HPB - 1) / HPB), n_tiles), 256 * HPB, lds, (hipStream_t)stream>>>( \
         (const elem_t*)q, q_stride, (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride,    \
-        positions, seq_rows, (elem_t*)out, tiles, n_heads, n_kv_heads, page_size, window, scale);                               \
+        positions, seq_rows, (elem_t*)out, tiles, partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);             \
   }
 #if AXON_BF16
-  // one query head a workgroup while such workgroups find a CU each; beyond that two, which share what is unpacked
-  if (group >= 2 && (long)n_tiles * n_heads > 256) {
+  // one query head a workgroup while two such workgroups a CU are enough; beyond that two, which share what is unpacked
+  if (group >= 2 && (long)n_tiles * n_heads > 512) {
     if (head_dim == 64) LAUNCH(64, 2) else LAUNCH(128, 2)
   } else
 #endif
@@ -943,5 +1054,12 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
   }
 #undef LAUNCH
   AXK_LAUNCH_CHECK("kv4_attention_prefill");
+  if (n_slots > 0) {
+    if (head_dim == 64)
+      kv4_fold_kernel<64><<<dim3(n_heads, n_tiles), 256, 0, (hipStream_t)stream>>>((elem_t*)out, tiles, partial, n_slots, n_heads);
+    else
+      kv4_fold_kernel<128><<<dim3(n_heads, n_tiles), 256, 0, (hipStream_t)stream>>>((elem_t*)out, tiles, partial, n_slots, n_heads);
+    AXK_LAUNCH_CHECK("kv4_attention_prefill");
+  }
   return 0;
 }

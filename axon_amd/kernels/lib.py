@@ -184,7 +184,7 @@ _SIGNATURES = {
     "axk_kv4_attention_decode": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                  c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
     "axk_kv4_attention_prefill": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                                  c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
+                                  c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
 }
 
 
@@ -192,7 +192,7 @@ _SIGNATURES = {
 _PLAIN = ["axk_argmax_workspace", "axk_attention_decode_chunk", "axk_attention_decode_item_factor", "axk_attention_decode_workspace",
           "axk_attention_prefill_tile", "axk_delta_chunked_workspace", "axk_gemm_workspace", "axk_latent_attention_workspace",
           "axk_masked_attention_workspace", "axk_packed_elems", "axk_kv4_decode_chunk", "axk_kv4_decode_item_factor",
-          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile"]
+          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile", "axk_kv4_prefill_segment", "axk_kv4_prefill_workspace"]
 
 
 def _calls_module():
@@ -265,6 +265,8 @@ class Kernels:
         self.lib.axk_delta_chunked_workspace.restype = ctypes.c_long
         self.lib.axk_kv4_decode_workspace.argtypes = [c_int] * 4
         self.lib.axk_kv4_decode_workspace.restype = ctypes.c_long
+        self.lib.axk_kv4_prefill_workspace.argtypes = [c_int] * 3
+        self.lib.axk_kv4_prefill_workspace.restype = ctypes.c_long
         self.lib.axk_packed_elems.argtypes = [c_int, c_int]
         self.lib.axk_packed_elems.restype = ctypes.c_long
         self.lib.axk_gemm_workspace.argtypes = [c_int, c_int, c_int, c_int]
@@ -1816,41 +1818,55 @@ class Kernels:
         return out
 
     def kv4_prefill_tiles(self, spans, window: int, n_heads: int, n_kv_heads: int) -> List[tuple]:
-        """The tiles of `kv4_attention_prefill` for portions (first token of the step, tokens, position of the first): rows of
-        (first, count, first, count), two runs of one request's tokens that a block takes one after the other."""
-        tile = int(self.run.axk_kv4_prefill_tile())
+        """The tiles of `kv4_attention_prefill` for portions (first token of the step, tokens, position of the first): rows of (first
+        token, count, segment, slot of the workspace), those with the most work first.  A tile whose rows see several segments of positions is
+        cut there where a step has few tiles (its segments then run side by side, and a last row has them folded); the bits are
+        the same either way."""
+        tile, segment = int(self.run.axk_kv4_prefill_tile()), int(self.run.axk_kv4_prefill_segment())
         runs = []
         for start, length, at in spans:
             if start < 0 or length < 1 or at < 0:
                 raise KernelError(f"kv4_attention_prefill: a portion of {length} tokens from token {start}, at position {at}")
             for first in range(0, length, tile):
                 n = min(tile, length - first)
-                last = at + first + n
-                runs.append((min(last, window + n) if window > 0 else last, start + first, n))
-        runs.sort(key=lambda r: -r[0])
-        rows = []
-        for i in range((len(runs) + 1) // 2):
-            other = runs[len(runs) - 1 - i][1:] if len(runs) - 1 - i > i else (0, 0)
-            rows.append(runs[i][1:] + other)
-        return rows
+                runs.append((start + first, n, max(0, at + first + 1 - window) if window > 0 else 0, at + first + n - 1))
+        # two workgroups of one head fit a CU: fewer than that, and tiles are cut (a tile at 30,000 positions alone takes 28 of 256 CUs
+        # 0.8 ms, and cut all of them 0.1)
+        cut = len(runs) * n_heads < 512
+        rows, folds, slots = [], [], 0
+        for start, n, low, high in runs:
+            first, last = low // segment, high // segment
+            if first == last:
+                rows.append((high - low, start, n, -1, -1))
+            elif not cut:
+                rows.append((high - low, start, n, -1, slots))
+                slots += 1
+            else:
+                rows += [(min(high, (s + 1) * segment - 1) - max(low, s * segment), start, n, s, slots + s - first) for s in range(first, last + 1)]
+                folds.append((start, n, -1 - (last - first + 1), slots))
+                slots += last - first + 1
+        rows.sort(key=lambda r: -r[0])
+        return [r[1:] for r in rows] + folds
 
     def kv4_prefill_workspace(self, tiles, n_heads: int, head_dim: int) -> int:
-        """Floats of `kv4_attention_prefill`'s workspace for these tiles."""
-        return 0
+        """Floats of `kv4_attention_prefill`'s workspace for these tiles (as `kv4_prefill_tiles` lists them)."""
+        slots = max((row[3] + (-1 - row[2] if row[2] < -1 else 1) for row in tiles), default=0)
+        return int(self.run.axk_kv4_prefill_workspace(slots, n_heads, head_dim))
 
     def kv4_attention_prefill(self, q, q_stride, k_cache, v_cache, block_table, positions, seq_rows, out, tiles, partial, n_heads,
                               n_kv_heads, head_dim, page_size, window, scale) -> torch.Tensor:
-        """`attention_prefill` over a cache held in 4 bits: prompt portions by `kv4_prefill_tiles` (int32 [n, 4] on the device);
-        rows of no tile are left as they are."""
+        """`attention_prefill` over a cache held in 4 bits: prompt portions by `kv4_prefill_tiles` (int32 [n, 4] on the device); partial:
+        float32, `kv4_prefill_workspace` of these tiles.  Rows of no tile are left as they are."""
         T = self._kv4_step("kv4_attention_prefill", k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size,
                            q, out, tiles, partial)
         self._kv4_rows("kv4_attention_prefill", q, q_stride, out, T, n_heads, head_dim)
-        self._i32(tiles, "tiles")
+        self._i32(tiles, "tiles"); self._f32(partial, "attention partial")
         if tiles.numel() and (tiles.dim() != 2 or tiles.shape[1] != 4):
             raise KernelError(f"kv4_attention_prefill: tiles {tuple(tiles.shape)}")
         self._check(self.run.axk_kv4_attention_prefill(
             _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[-1], _ptr(positions), _ptr(seq_rows),
-            _ptr(out), _ptr(tiles), tiles.numel() // 4, n_heads, n_kv_heads, head_dim, page_size, window, float(scale), _queue()))
+            _ptr(out), _ptr(tiles), tiles.numel() // 4, _ptr(partial), partial.numel(), n_heads, n_kv_heads, head_dim, page_size, window,
+            float(scale), _queue()))
         return out
 
     def fill_i32(self, dst: torch.Tensor, value: int) -> None:

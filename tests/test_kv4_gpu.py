@@ -323,6 +323,63 @@ def test_prefill(dtype, spans, nh, nkv, dim, page, window):
         assert torch.equal(torch.cat(parts), whole)
 
 
+def prefill_by(k, held, q, tiles, pos, seq, nh, nkv, dim, page, window, scale):
+    out = torch.full((len(pos), nh * dim), 5.0, dtype=q.dtype, device="cuda")
+    partial = torch.full((k.kv4_prefill_workspace(tiles, nh, dim),), float("nan"), device="cuda")
+    return k.kv4_attention_prefill(q, q.stride(0), *held.args, i32(pos), i32(seq), out, i32(tiles), partial, nh, nkv, dim, page, window, scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,at,nh,nkv,dim,window", [(70, 4090, 2, 1, 64, 0), (131, 1990, 3, 1, 128, 0), (40, 5000, 2, 2, 128, 2500), (3, 2047, 4, 1, 64, 2048)])
+def test_tiles_cut_at_segments(dtype, n, at, nh, nkv, dim, window):
+    """Positions beyond a segment: the segments side by side and folded, or all by one workgroup: the same bits, and right."""
+    k, page, held = kernels(dtype), 32, Held([n + at], nkv, dim, 32, seed=11)
+    q = torch.randn((n, nh * dim), generator=torch.Generator().manual_seed(4)).to(TORCH[dtype]).cuda()
+    pos, seq = list(range(at, at + n)), [0] * n
+    cut = k.kv4_prefill_tiles([(0, n, at)], window, nh, nkv)
+    assert any(row[2] < -1 for row in cut) and any(row[2] >= 0 for row in cut)
+    got = prefill_by(k, held, q, cut, pos, seq, nh, nkv, dim, page, window, 0.1)
+    whole = prefill_by(k, held, q, [(f, min(128, n - f), -1, i) for i, f in enumerate(range(0, n, 128))], pos, seq, nh, nkv, dim, page, window, 0.1)
+    assert torch.equal(got, whole)
+    some = [0, n // 2, n - 1]
+    check(dtype, got[some], q[some], held, [pos[i] for i in some], [0] * 3, window, 0.1, dim, nh)
+    # a slot that is not there: nothing is read or written behind the workspace, the tile's rows stay as they were
+    empty = torch.empty(0, device="cuda")
+    out = torch.full_like(q, 5.0)
+    k.kv4_attention_prefill(q, q.stride(0), *held.args, i32(pos), i32(seq), out, i32(cut), empty, nh, nkv, dim, page, window, 0.1)
+    assert (out == 5.0).all()
+
+
+@pytest.mark.parametrize("nh,nkv,dim,portions", [(14, 2, 64, 40), (28, 4, 128, 20), (9, 3, 128, 60), (5, 1, 64, 110)])
+def test_two_heads_a_workgroup(nh, nkv, dim, portions):
+    """Steps of many tiles: a workgroup has two heads of a key head (an odd group leaves one out); the same bits as few tiles give."""
+    k, page = kernels("bfloat16"), 16
+    lengths = [(i * 37) % 90 + 2 for i in range(portions)]
+    spans = [((i * 13) % n + 1, n - (i * 13) % n - 1) for i, n in enumerate(lengths)]
+    held = Held(lengths, nkv, dim, page, seed=12)
+    T = sum(n for n, _ in spans)
+    q = torch.randn((T, nh * dim), generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    k.reset_instances()
+    pos, seq, got = prefill(k, held, q, spans, range(portions), nh, nkv, dim, page, 0, 0.1)
+    assert k.instances(launched=True) == [f"kv4_prefill<{dim},2>"]
+    first = 0
+    for r, (n, at) in enumerate(spans):
+        if r % 7 == 0:
+            one = prefill(k, held, q[first:first + n], [(n, at)], [r], nh, nkv, dim, page, 0, 0.1)[2]
+            assert torch.equal(one, got[first:first + n])
+        first += n
+    some = list(range(0, T, max(1, T // 12)))
+    check("bfloat16", got[some], q[some], held, [pos[i] for i in some], [seq[i] for i in some], 0, 0.1, dim, nh)
+    # longer than a segment
+    held = Held([2300], nkv, dim, page, seed=13)
+    tiles, n, at = [], 20, 2280
+    q = torch.randn((n, nh * dim), generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    pos, seq = list(range(at, at + n)), [0] * n
+    alone = prefill_by(k, held, q, [(0, n, -1, 0)], pos, seq, nh, nkv, dim, page, 0, 0.1)
+    many = prefill_by(k, held, q, [(0, n, -1, 0)] + [(0, 0, -1, -1)] * (513 // nh + 1), pos, seq, nh, nkv, dim, page, 0, 0.1)
+    assert torch.equal(alone, many)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scores_of_any_size_and_queries_of_zero(dtype):
     """Queries from 2^-60 to 2^60 times the ordinary, and a query of zeros: the softmax is as sharp as it should be."""
