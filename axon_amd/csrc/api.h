@@ -536,11 +536,12 @@ int axk_kv4_attention_decode(const void* q, int q_stride, const void* k_cache, c
                              int max_chunks, int n_heads, int n_kv_heads, int head_dim, int page_size, int window, float scale,
                              void* stream);
 // Prompt portions: tiles [n_tiles][4] = (first token, count up to axk_kv4_prefill_tile, segment, slot).  segment -1: everything that the
-// tile's rows see, which needs a slot of the workspace (its own, else -1) if that reaches over a multiple of axk_kv4_prefill_segment positions;
-// segment s: only positions s x axk_kv4_prefill_segment and up to the next, into its slot; segment -1 - n: the tile's n segments, which lie in
+// tile's rows see, which needs a slot of the workspace (its own, else -1) if that lies in several segments of positions
+// (axk_kv4_prefill_segment); segment s: only the positions from axk_kv4_prefill_segment_start(s) up to the next, into its slot; segment -1 - n: the tile's n segments, which lie in
 // n slots from `slot` on, are folded into its rows of out (by a second launch).  The same bits either way.
 int axk_kv4_prefill_tile(void);
-int axk_kv4_prefill_segment(void);
+int axk_kv4_prefill_segment(int position);
+int axk_kv4_prefill_segment_start(int segment);
 long axk_kv4_prefill_workspace(int n_slots, int n_heads, int head_dim);
 int axk_kv4_attention_prefill(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int32_t* block_table,
                               int table_stride, const int32_t* positions, const int32_t* seq_rows, void* out, const int32_t* tiles,

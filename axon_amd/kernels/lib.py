@@ -192,7 +192,8 @@ _SIGNATURES = {
 _PLAIN = ["axk_argmax_workspace", "axk_attention_decode_chunk", "axk_attention_decode_item_factor", "axk_attention_decode_workspace",
           "axk_attention_prefill_tile", "axk_delta_chunked_workspace", "axk_gemm_workspace", "axk_latent_attention_workspace",
           "axk_masked_attention_workspace", "axk_packed_elems", "axk_kv4_decode_chunk", "axk_kv4_decode_item_factor",
-          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile", "axk_kv4_prefill_segment", "axk_kv4_prefill_workspace"]
+          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile", "axk_kv4_prefill_segment",
+          "axk_kv4_prefill_segment_start", "axk_kv4_prefill_workspace"]
 
 
 def _calls_module():
@@ -1822,7 +1823,8 @@ class Kernels:
         token, count, segment, slot of the workspace), those with the most work first.  A tile whose rows see several segments of positions is
         cut there where a step has few tiles (its segments then run side by side, and a last row has them folded); the bits are
         the same either way."""
-        tile, segment = int(self.run.axk_kv4_prefill_tile()), int(self.run.axk_kv4_prefill_segment())
+        tile = int(self.run.axk_kv4_prefill_tile())
+        segment_of, start_of = self.run.axk_kv4_prefill_segment, self.run.axk_kv4_prefill_segment_start
         runs = []
         for start, length, at in spans:
             if start < 0 or length < 1 or at < 0:
@@ -1831,18 +1833,19 @@ class Kernels:
                 n = min(tile, length - first)
                 runs.append((start + first, n, max(0, at + first + 1 - window) if window > 0 else 0, at + first + n - 1))
         # two workgroups of one head fit a CU: fewer than that, and tiles are cut (a tile at 30,000 positions alone takes 28 of 256 CUs
-        # 0.8 ms, and cut all of them 0.1)
+        # 0.8 ms, and cut 0.2)
         cut = len(runs) * n_heads < 512
         rows, folds, slots = [], [], 0
         for start, n, low, high in runs:
-            first, last = low // segment, high // segment
+            first, last = int(segment_of(low)), int(segment_of(high))
             if first == last:
                 rows.append((high - low, start, n, -1, -1))
             elif not cut:
                 rows.append((high - low, start, n, -1, slots))
                 slots += 1
             else:
-                rows += [(min(high, (s + 1) * segment - 1) - max(low, s * segment), start, n, s, slots + s - first) for s in range(first, last + 1)]
+                rows += [(min(high, int(start_of(s + 1)) - 1) - max(low, int(start_of(s))), start, n, s, slots + s - first)
+                         for s in range(first, last + 1)]
                 folds.append((start, n, -1 - (last - first + 1), slots))
                 slots += last - first + 1
         rows.sort(key=lambda r: -r[0])

@@ -330,7 +330,8 @@ def prefill_by(k, held, q, tiles, pos, seq, nh, nkv, dim, page, window, scale):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,at,nh,nkv,dim,window", [(70, 4090, 2, 1, 64, 0), (131, 1990, 3, 1, 128, 0), (40, 5000, 2, 2, 128, 2500), (3, 2047, 4, 1, 64, 2048)])
+@pytest.mark.parametrize("n,at,nh,nkv,dim,window", [(70, 8150, 2, 1, 64, 0), (131, 1990, 3, 1, 128, 0), (40, 16390, 2, 2, 128, 9000),
+                                                    (3, 2047, 4, 1, 64, 2048)])
 def test_tiles_cut_at_segments(dtype, n, at, nh, nkv, dim, window):
     """Positions beyond a segment: the segments side by side and folded, or all by one workgroup: the same bits, and right."""
     k, page, held = kernels(dtype), 32, Held([n + at], nkv, dim, 32, seed=11)
