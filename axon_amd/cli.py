@@ -52,6 +52,7 @@ def _engine_flags(p: argparse.ArgumentParser) -> None:
     p.add_argument("--dtype", default="bfloat16", help="bfloat16 (default) or float32: true 32-bit everywhere")
     p.add_argument("--ctx", type=int, default=0, help="positions a request may reach (default: the model's)")
     p.add_argument("--page-size", type=int, default=64, help="positions in one cache page (default 64: a block of the attention kernels)")
+    p.add_argument("--cache-bits", type=int, default=0, choices=[0, 4], help="4: keys and values held in 4 bits (default 0: in the dtype)")
     p.add_argument("--num-pages", type=int, default=0, help="pages in the cache pool (default: what the request needs)")
     p.add_argument("--device", default="cuda:0", help="the GPU to run on (default cuda:0)")
     p.add_argument("--random-weights", type=int, default=None, metavar="SEED",
@@ -123,7 +124,7 @@ def _load(args, need_tokens: int, requests: int = 1):
         _refuse(f"the prompt and the tokens to generate need {need_tokens} positions, the context is {ctx}")
     pages = args.num_pages or requests * (-(-need_tokens // args.page_size) + 1)
     settings = dict(dtype=args.dtype, device=args.device, page_size=args.page_size, num_pages=pages,
-                    max_seqs=max(2, requests), max_seq_len=ctx, max_batch_tokens=2048)
+                    max_seqs=max(2, requests), max_seq_len=ctx, max_batch_tokens=2048, cache_bits=args.cache_bits)
     if args.random_weights is not None:
         llm = axon_amd.load(cfg, random_seed=args.random_weights, init_std=args.std, **settings)
     else:

@@ -323,17 +323,18 @@ class LLM:
 def load(model: Union[str, dict, ModelConfig], dtype: str = "bfloat16", *, random_seed: Optional[int] = None,
          init_std: float = 0.02, device: str = "cuda:0", page_size: int = 64, num_pages: int = 0,
          max_cache_tokens: int = 0, memory_fraction: float = 0.85, max_seqs: int = 64, max_batch_tokens: int = 2048,
-         max_seq_len: int = 0, use_graphs: bool = True) -> LLM:
+         max_seq_len: int = 0, use_graphs: bool = True, cache_bits: int = 0) -> LLM:
     """A model folder (config.json + safetensors), or a configuration (a dict of config.json
-    keys or a ModelConfig) with `random_seed` for random weights, to a ready `LLM`."""
+    keys or a ModelConfig) with `random_seed` for random weights, to a ready `LLM`.  `cache_bits` 4: keys and values of
+    grouped-query attention are held in 4 bits (4.5 with their scales) instead of the compute dtype."""
     rt = Runtime(dtype, device)
     if isinstance(model, str):
-        m = load_model(model, rt)
+        m = load_model(model, rt, cache_bits)
     else:
         config = config_from_dict(model) if isinstance(model, dict) else model
         if random_seed is None:
             raise ValueError("a configuration without a model folder needs random_seed")
-        m = random_model(config, rt, random_seed, init_std)
+        m = random_model(config, rt, random_seed, init_std, cache_bits)
     cfg = EngineConfig(dtype=dtype, page_size=page_size, num_pages=num_pages, max_cache_tokens=max_cache_tokens,
                        memory_fraction=memory_fraction, max_seqs=max_seqs, max_batch_tokens=max_batch_tokens,
                        max_seq_len=max_seq_len, use_graphs=use_graphs)

@@ -30,10 +30,10 @@ def read_model_config(model_dir: str, checkpoint: Optional[Checkpoint] = None) -
     return config
 
 
-def load_model(model_dir: str, rt: Runtime) -> DecoderModel:
+def load_model(model_dir: str, rt: Runtime, cache_bits: int = 0) -> DecoderModel:
     ck = Checkpoint(model_dir)
     config = read_model_config(model_dir, ck)
-    model = build_model_description(config)
+    model = build_model_description(config, cache_bits)
     source = CheckpointSource(ck)
     check_tensors(model.tensors(), source, config.ignores_tensor)
     model.load(WeightStore(source, rt.device, rt.dtype), rt)
@@ -41,9 +41,9 @@ def load_model(model_dir: str, rt: Runtime) -> DecoderModel:
     return model
 
 
-def random_model(config: ModelConfig, rt: Runtime, seed: int = 0, std: float = 0.02) -> DecoderModel:
+def random_model(config: ModelConfig, rt: Runtime, seed: int = 0, std: float = 0.02, cache_bits: int = 0) -> DecoderModel:
     """A model whose weights are drawn on the device (nothing is written)."""
-    model = build_model_description(config)
+    model = build_model_description(config, cache_bits)
     storage = torch.bfloat16 if rt.dtype == torch.bfloat16 else torch.float32
     source = RandomSource(model.tensors(), seed, std=std, storage=storage)
     model.load(WeightStore(source, rt.device, rt.dtype), rt)

@@ -113,6 +113,8 @@ class Engine:
             limit = b.mixer.max_context()
             if limit is not None and self.max_seq_len > limit:
                 raise StepError(f"max_seq_len {self.max_seq_len}: a mixer of this model takes contexts of up to {limit}")
+            if not b.mixer.takes_page_size(cfg.page_size):
+                raise StepError(f"page_size {cfg.page_size}: a mixer of this model takes other cache pages (its kernels: powers of two from 8 to 1024)")
         # workspaces mixers want in decoding steps (Mixer.decode_scratch): one per name, sized for the
         # most requests and the longest context, allocated at the first decoding step (the pool leaves room for them)
         self._scratch_sizes: Dict = {}

@@ -1766,6 +1766,14 @@ class Kernels:
             raise KernelError(f"kv4_attention_decode: a context of {int(pos.max()) + 1} positions, at most {self.kv4_max_context}")
         return n
 
+    def kv4_most_chunks(self, max_seq_len: int, window: int) -> int:
+        """The most chunks that a token of a request of up to `max_seq_len` positions sees: not the longest's, where chunks grow."""
+        most, longest = 1, min(max_seq_len, window) if window > 0 else max_seq_len
+        self._kv4_chunk_sizes(1)
+        for seen in [longest] + [int(start) - 1 for start in self._kv4_steps[0] if 1 < start <= longest]:
+            most = max(most, -(-seen // int(self._kv4_chunk_sizes(seen))) + (1 if window > 0 else 0))
+        return most
+
     def kv4_decode_chunks(self, positions: Sequence[int], window: int) -> int:
         """The most chunks that any token at these positions sees (1 at least): `max_chunks` of the workspace and the call."""
         return int(self._kv4_chunk_counts(positions, window).max(initial=1))

@@ -24,8 +24,11 @@ class CachePlan:
 
 
 class DecoderModel:
-    def __init__(self, config: ModelConfig):
+    def __init__(self, config: ModelConfig, cache_bits: int = 0):
+        if cache_bits not in (0, 4):
+            raise ConfigError(f"cache_bits {cache_bits!r} is not 0 (the compute dtype) or 4")
         self.config = config
+        self.cache_bits = cache_bits
         spec = config.model_spec()
         self.spec = spec
         self.hidden_size = spec.hidden_size
@@ -37,7 +40,11 @@ class DecoderModel:
             mixer = build_part("mixer", layer.mixer, layer.prefix)
             # a layer may have no feed-forward (its block then has to be one that takes none)
             ffn = build_part("feed_forward", layer.feed_forward, layer.prefix) if layer.feed_forward is not None else None
+            if cache_bits:
+                mixer.hold_cache_in(cache_bits)
             self.blocks.append(build_block(layer.block, layer.norm, mixer, ffn, layer.prefix))
+        if cache_bits and all(b.mixer.cache_spec() is None for b in self.blocks):
+            raise ConfigError(f"cache_bits {cache_bits}: no mixer of this model keeps keys and values")
         # rewrites of the residual stream that runs may enter through (they read the embedding's output)
         self.entries = [build_part("stream", e) for e in spec.entries]
         self.final_norm = build_part("norm", spec.final_norm)

@@ -11,6 +11,12 @@ The three projections run as one product over a fused [q_dim + 2 kv_dim, hidden]
 
 Parameters: `hidden_size`, `num_heads`, `num_kv_heads`, `head_dim`, `qkv_bias` (True, False
 or "optional"), `out_bias`, `window` (0: all earlier positions), `position` (a PartSpec).
+
+`hold_cache_in(4)`: keys and values in 4 bits with a scale and a zero for 32 dims (head sizes 64 and 128).  The
+projection is then a plain product, the rotation quantises what it stores, and portions of up to 16 tokens go token by token.
+A token's bits do not depend on what else is in a step, and a portion's not on how it is cut into larger ones; but the kernel for
+single tokens and the one for portions sum in orders of their own, so a position that came as a single token (or was decoded) and the same one in
+a portion of more agree within their rounding, not bit for bit.
 """
 from __future__ import annotations
 
@@ -159,6 +165,39 @@ def decode_scratch_floats(k, window: int, n_heads: int, head_dim: int, max_seqs:
     return k.attention_decode_workspace(max_seqs, n_heads, head_dim, 1 << (most - 1).bit_length())
 
 
+KV4_SINGLES = 16        # portions of up to so many tokens go token by token to the 4-bit cache's kernel for single tokens
+
+
+class Kv4Plan:
+    """How the 4-bit cache's kernels split a step: portions of more than 16 tokens by tiles, the others token by token (16 tokens at
+    4,000 positions 17 us so, 60 by a tile; by its length alone, so that a portion's bits do not depend on the step).  Made once per
+    step and window, shared by all layers."""
+
+    def __init__(self, ctx, window: int, n_heads: int, n_kv_heads: int, head_dim: int):
+        k, dev = ctx.rt.k, ctx.rt.device
+        self.tiles = self.tile_partial = self.decode_tokens = None
+        if ctx.decode_only:
+            self.decode_tokens = ctx.n_tokens
+            self.max_chunks = ctx.decode_shapes[("kv4_chunks", window)]
+            self.decode_work = ctx.decode_inputs[("kv4_work", window)]
+            self.partial = ctx.decode_scratch[("kv4_partial", window, n_heads, head_dim)]
+            return
+        if any(s.q_len < 1 or s.q_start < 0 or s.q_start + s.q_len > ctx.n_tokens for s in ctx.spans):
+            raise ValueError("attention plan: a span lies outside the tokens of the step")
+        short = [s for s in ctx.spans if s.q_len <= KV4_SINGLES]
+        portions = [(s.q_start, s.q_len, s.start_pos) for s in ctx.spans if s.q_len > KV4_SINGLES]
+        if portions:
+            rows = k.kv4_prefill_tiles(portions, window, n_heads, n_kv_heads)
+            self.tiles = upload(rows, dev)
+            self.tile_partial = torch.empty(k.kv4_prefill_workspace(rows, n_heads, head_dim), dtype=torch.float32, device=dev)
+        if short:
+            at = [s.start_pos + i for s in short for i in range(s.q_len)]
+            self.decode_tokens = upload([s.q_start + i for s in short for i in range(s.q_len)], dev)
+            self.max_chunks = k.kv4_decode_chunks(at, window)
+            self.decode_work = upload(k.kv4_decode_work(at, window), dev)
+            self.partial = torch.empty(k.kv4_decode_workspace(len(at), n_heads, head_dim, self.max_chunks), dtype=torch.float32, device=dev)
+
+
 class GQAttention(Mixer):
     graph_safe = True
     def __init__(self, params, prefix=""):
@@ -182,6 +221,7 @@ class GQAttention(Mixer):
         base = prefix + names.get("scope", "self_attn.")
         self.n = {k: base + names.get(k, k + "_proj") for k in ("q", "k", "v", "o")}
         self.w_qkv = self.b_qkv = self.w_o = self.b_o = None
+        self.cache_bits = 0                  # 0: in the compute dtype
         self._max_context = None
         self._kernels = None                 # those that want a workspace in decoding steps
         self.decode_chunk = 1 << 30          # until `load` has asked the kernels: one chunk
@@ -202,7 +242,20 @@ class GQAttention(Mixer):
             t.append(TensorDecl(self.n["o"] + ".bias", (self.hidden,), "bias"))
         return t
 
+    def hold_cache_in(self, bits: int) -> None:
+        if bits != 4 or self.hd not in (64, 128):
+            raise ConfigError(f"a cache in {bits} bits of heads of {self.hd}: there are 4 bits, for heads of 64 and 128")
+        if self.position is not None and self.position.rotary_dim % 16:
+            raise ConfigError(f"a cache in {bits} bits rotates a multiple of 16 dims, not {self.position.rotary_dim}")
+        self.cache_bits = bits
+
+    def takes_page_size(self, page_size: int) -> bool:
+        return self.cache_bits == 0 or self._kernels is None or self._kernels.kv4_ok(self.hd, page_size)
+
     def cache_spec(self) -> Optional[CacheSpec]:
+        if self.cache_bits:
+            # half a byte a number, and a scale of two bytes for 32 of them
+            return CacheSpec(entries=2, heads=self.nkv, head_dim=self.hd // 2 + self.hd // 16, window=self.window, dtype="uint8")
         return CacheSpec(entries=2, heads=self.nkv, head_dim=self.hd, window=self.window)
 
     def max_context(self):
@@ -212,6 +265,9 @@ class GQAttention(Mixer):
         """The decoding kernel's workspace is laid out by the longest context of the step, in
         chunks of the kernel's size, rounded up to a power of two so that few shapes exist (the
         blocks that are launched are those of `decode_input`, whatever this number)."""
+        if self.cache_bits:
+            most = self._kernels.kv4_decode_chunks(positions, self.window)
+            return ("kv4_chunks", self.window), 1 << (most - 1).bit_length()
         most = max(decode_chunks_of(p, self.window, self.decode_chunk) for p in positions)
         return ("attention_chunks", self.window), 1 << (most - 1).bit_length()
 
@@ -220,15 +276,22 @@ class GQAttention(Mixer):
         for the chunks that exist, not for the longest context times the tokens.  Padded in
         steps of an eighth or less."""
         work = self._work_list(positions, self.window)
-        return ("attention_work", self.window), work + [-1] * (round_up_by_eighths(len(work)) - len(work))
+        name = "kv4_work" if self.cache_bits else "attention_work"
+        return (name, self.window), work + [-1] * (round_up_by_eighths(len(work)) - len(work))
 
     def decode_input_capacity(self, max_seqs: int, max_seq_len: int) -> int:
+        if self.cache_bits:
+            return round_up_by_eighths(max_seqs * self._kernels.kv4_most_chunks(max_seq_len, self.window))
         return round_up_by_eighths(max_seqs * decode_chunks_of(max(0, max_seq_len - 1), 0, self.decode_chunk))
 
     def decode_scratch(self, max_seqs: int, max_seq_len: int):
         """The blocks' partial results of the decoding kernel (see `decode_shape`)."""
         if self._kernels is None:                # no kernel of this build and these sizes wants one
             return None
+        if self.cache_bits:
+            chunks = self._kernels.kv4_most_chunks(max_seq_len, self.window)
+            return (("kv4_partial", self.window, self.nh, self.hd),
+                    self._kernels.kv4_decode_workspace(max_seqs, self.nh, self.hd, 1 << (chunks - 1).bit_length()))
         floats = decode_scratch_floats(self._kernels, self.window, self.nh, self.hd, max_seqs, max_seq_len)
         if floats > FLOAT32_PARTIAL and not self._kernels.attention_fast_ok(self.hd, 64, self.nh, self.nkv):
             return None
@@ -240,6 +303,10 @@ class GQAttention(Mixer):
         self._max_context = rt.k.attention_decode_max_context
         if rt.k.attention_blocks_ok(self.hd, 64, self.nh, self.nkv):
             self._kernels = rt.k
+        if self.cache_bits:
+            if not rt.k.kv4_ok(self.hd, 64) or self.cache_spec().head_dim != rt.k.kv4_row_bytes(self.hd):
+                raise ConfigError(f"{self.prefix}: the 4-bit cache's kernels do not take heads of {self.hd}")
+            self._kernels, self._work_list, self._max_context = rt.k, rt.k.kv4_decode_work, rt.k.kv4_max_context
         self.w_qkv = rt.k.prepare_weight(store.fused_matrix([self.n[k] + ".weight" for k in ("q", "k", "v")]))
         biases = [store.vector(self.n[k] + ".bias", optional=True) for k in ("q", "k", "v")] if self.qkv_bias else []
         present = [b is not None for b in biases]
@@ -261,7 +328,7 @@ class GQAttention(Mixer):
     def applies_preceding_norm(self, ctx) -> bool:
         k = ctx.rt.k
         rows = self.q_dim + 2 * self.kv_dim
-        return (isinstance(self.w_qkv, PackedMatrix) and self.position is not None
+        return (isinstance(self.w_qkv, PackedMatrix) and self.position is not None and not self.cache_bits
                 and k.gemm_qkv_rope_ok(ctx.n_tokens, rows, self.hidden, self.hd, self.position.rotary_dim)
                 and k.gemm_normed_ok(ctx.n_tokens, rows, self.hidden))
 
@@ -270,6 +337,9 @@ class GQAttention(Mixer):
         T = h.shape[0]
         group = ctx.cache.group(binding.group)
         k_cache, v_cache = group.layer(binding.index)
+        if self.cache_bits:
+            self._forward_kv4(ctx, group, k_cache, v_cache, binding.writes, h, residual, following)
+            return
         # values are kept position-contiguous: a page of them is [heads, head_dim, page_size]
         v_cache = v_cache.view(v_cache.shape[0], self.nkv, self.hd, group.page_size)
         qkv = ctx.ws.take((T, self.q_dim + 2 * self.kv_dim), ctx.rt.dtype)
@@ -310,6 +380,33 @@ class GQAttention(Mixer):
         else:
             k.attention(qkv, qkv.stride(0), k_cache, v_cache, group.block_table, ctx.positions, ctx.seq_rows, att,
                         self.nh, self.nkv, self.hd, group.page_size, self.window, self.scale)
+        k.gemm(att, self.w_o, residual, self.b_o, MODE_ADD_F32,
+               following_norm=None if following is None else following.as_argument())
+
+
+    def _forward_kv4(self, ctx, group, k_cache, v_cache, writes, h, residual, following) -> None:
+        k, T = ctx.rt.k, h.shape[0]
+        if isinstance(h, PrecedingNorm):
+            h = h.apply(ctx)
+        table, rotary = (self.position.tables(ctx), self.position.rotary_dim) if self.position is not None else (ctx.no_rotation(), 0)
+        width = self.q_dim + (2 * self.kv_dim if writes else 0)
+        qkv = ctx.ws.take((T, width), ctx.rt.dtype)
+        k.gemm(h, self.w_qkv[:width], qkv, None if self.b_qkv is None else self.b_qkv[:width], MODE_STORE)
+        q = qkv[:, :self.q_dim]
+        sizes = (self.nh, self.nkv, self.hd)
+        k.rope_kv4_write(qkv, q, table, ctx.positions, ctx.seq_rows, group.block_table, k_cache, v_cache, *sizes, rotary,
+                         group.page_size, writes)
+        att = ctx.ws.take((T, self.q_dim), ctx.rt.dtype)
+        key = ("kv4_plan", self.window, *sizes)
+        if key not in ctx.shared:
+            ctx.shared[key] = Kv4Plan(ctx, self.window, *sizes)
+        plan = ctx.shared[key]
+        common = (q, qkv.stride(0), k_cache, v_cache, group.block_table, ctx.positions, ctx.seq_rows, att)
+        if plan.tiles is not None:
+            k.kv4_attention_prefill(*common, plan.tiles, plan.tile_partial, *sizes, group.page_size, self.window, self.scale)
+        if plan.decode_tokens is not None:
+            k.kv4_attention_decode(*common, plan.decode_tokens, plan.partial, plan.max_chunks, *sizes, group.page_size, self.window,
+                                   self.scale, work=plan.decode_work)
         k.gemm(att, self.w_o, residual, self.b_o, MODE_ADD_F32,
                following_norm=None if following is None else following.as_argument())
 

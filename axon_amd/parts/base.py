@@ -180,6 +180,16 @@ class Mixer(Part):
         spec = self.state_spec()
         return [] if spec is None else [spec]
 
+    def hold_cache_in(self, bits: int) -> None:
+        """Keep the keys and values of the paged cache in `bits` bits a number (asked before anything is loaded or planned).  A mixer
+        without such a cache has nothing to do; one that can only hold it in the compute dtype refuses."""
+        if self.cache_spec() is not None:
+            raise ConfigError(f"{type(self).__name__} does not hold its cache in {bits} bits")
+
+    def takes_page_size(self, page_size: int) -> bool:
+        """Whether the mixer's kernels take cache pages of so many positions.  The engine refuses others when it is built."""
+        return True
+
     def max_context(self) -> Optional[int]:
         """The most positions of a request this mixer's kernels take (None: no limit of its own).
         The engine refuses a longer `max_seq_len` when it is built, not in the middle of a step."""
