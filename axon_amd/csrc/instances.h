@@ -44,8 +44,6 @@ enum {
   INST_GATED_SCAN,           // 1: waves that feed the walk, 0: a thread a channel
   INST_MASKED_BLOCKS,        // maps, tiles of 16 value dims, chunks of 32 key dims: blocks of positions side by side
   INST_MASKED_FOLD,          // maps, value dims a lane
-  INST_KV4_DECODE,           // head_dim
-  INST_KV4_PREFILL,          // head_dim, query heads a workgroup
   INST_KINDS
 };
 

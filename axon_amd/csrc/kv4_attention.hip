@@ -10,7 +10,6 @@
 
 #include "api.h"
 #include "common.h"
-#include "instances.h"
 #include "kv4.h"
 
 #define KV4_BLOCK 64               // positions of a block: one pass of products
@@ -985,7 +984,6 @@ extern "C" int axk_kv4_attention_decode(const void* q, int q_stride, const void*
   const dim3 units(n_kv_heads * sets, n_work < 65535 ? n_work : 65535, (n_work + 65534) / 65535);
 #define LAUNCH(HD)                                                                                                              \
   {                                                                                                                             \
-    AXK_INSTANCE(INST_KV4_DECODE, HD);                                                                                          \
     kv4_decode_kernel<HD><<<units, 64 * KV4_WAVES, 0, (hipStream_t)stream>>>(                                                               \
         (const elem_t*)q, q_stride, (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride,    \
         positions, seq_rows, (elem_t*)out, token_index, n_tokens, work, n_work, partial, max_chunks, n_heads, n_kv_heads, sets, \
@@ -1042,7 +1040,6 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
       }                                                                                                                         \
       configured = true;                                                                                                        \
     }                                                                                                                           \
-    AXK_INSTANCE(INST_KV4_PREFILL, HD, HPB);                                                                                    \
     kv4_prefill_kernel<HD, HPB><<<dim3(n_kv_heads * ((group + HPB - 1) / HPB), n_tiles), 256 * HPB, lds, (hipStream_t)stream>>>( \
         (const elem_t*)q, q_stride, (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride,    \
         positions, seq_rows, (elem_t*)out, tiles, partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);             \

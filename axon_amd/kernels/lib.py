@@ -285,6 +285,7 @@ class Kernels:
         self._extensions: Dict[str, ctypes.CDLL] = {}      # a registered source's path -> its library
         self._chunk_factor = None
         self._kv4_steps = None
+        self._kv4_bytes: Dict = {}
 
     def _callables(self):
         """The library's entry points as the methods call them: bound natively where that module is there (csrc/host/calls.cpp), else
@@ -1686,22 +1687,29 @@ class Kernels:
 
     def _kv4_step(self, what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, *others) -> int:
         """The checks that the 4-bit cache's calls share; the number of tokens."""
-        self._i32(positions, "positions"); self._i32(seq_rows, "seq_rows"); self._i32(block_table, "block_table")
-        if not self.kv4_ok(head_dim, page_size):
+        # (in few calls of torch: these run before every launch of a step that takes some 10 us; a tensor of the host is on device -1)
+        row = self._kv4_bytes.get((head_dim, page_size))
+        if row is None:
+            row = self._kv4_bytes[head_dim, page_size] = self.kv4_row_bytes(head_dim) if self.kv4_ok(head_dim, page_size) else 0
+        if row == 0:
             raise KernelError(f"{what}: head_dim {head_dim} and pages of {page_size} positions are not taken by the 4-bit cache")
+        here = torch.cuda.current_device() if _raw_stream is None else torch._C._cuda_getDevice()
+        for t in (positions, seq_rows, block_table):
+            if t.dtype is not torch.int32 or t.get_device() != here or not t.is_contiguous():
+                raise KernelError(f"{what}: expected contiguous int32 tensors on cuda:{here}, got {t.dtype} on {t.device}")
         if positions.dim() != 1 or seq_rows.shape != positions.shape or block_table.dim() != 2:
             raise KernelError(f"{what}: positions {tuple(positions.shape)}, seq_rows {tuple(seq_rows.shape)}, block_table {tuple(block_table.shape)}")
-        here = torch.cuda.current_device()
         if k_cache is not None:
-            shape = (n_kv_heads, page_size, self.kv4_row_bytes(head_dim))
-            for cache in (k_cache, v_cache):
-                if (cache.dtype != torch.uint8 or not cache.is_cuda or cache.dim() != 4 or tuple(cache.shape[1:]) != shape
-                        or cache.shape[0] != k_cache.shape[0] or not cache.is_contiguous()):
-                    raise KernelError(f"{what}: a cache {tuple(cache.shape)} of {cache.dtype} is not uint8 [pages, {shape[0]}, {shape[1]}, {shape[2]}]")
-            if k_cache.numel() > 1 << 37:                    # places in it are 32-bit numbers of 32 bytes
+            shape = k_cache.shape
+            if (shape[1:] != (n_kv_heads, page_size, row) or v_cache.shape != shape or k_cache.dtype is not torch.uint8
+                    or v_cache.dtype is not torch.uint8 or not k_cache.is_contiguous() or not v_cache.is_contiguous()
+                    or k_cache.get_device() != here or v_cache.get_device() != here):
+                raise KernelError(f"{what}: caches {tuple(shape)} and {tuple(v_cache.shape)} of {k_cache.dtype} and {v_cache.dtype} on {k_cache.device} "
+                                  f"and {v_cache.device} are not uint8 [pages, {n_kv_heads}, {page_size}, {row}] on cuda:{here}")
+            if k_cache.numel() > 1 << 37:                        # places in it are 32-bit numbers of 32 bytes
                 raise KernelError(f"{what}: a cache of {k_cache.numel()} bytes, at most {1 << 37}")
-        for t in (positions, seq_rows, block_table, k_cache, v_cache, *others):
-            if t is not None and t.device.index != here:
+        for t in others:
+            if t.get_device() != here:
                 raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
         return positions.numel()
 
@@ -1791,14 +1799,18 @@ class Kernels:
         return int(self.run.axk_kv4_decode_workspace(n_tokens, n_heads, head_dim, max_chunks))
 
     def _kv4_rows(self, what, q, q_stride, out, T, n_heads, head_dim) -> None:
-        self._elem(q, what + " q"); self._elem(out, what + " out")
-        if q.dim() < 1 or q.stride(-1) != 1 or (T > 0 and q.numel() == 0):
-            raise KernelError(f"{what}: q {tuple(q.shape)}")
-        if T > 0 and (q_stride < n_heads * head_dim or q.untyped_storage().nbytes() // q.element_size() - q.storage_offset()
-                      < (T - 1) * q_stride + n_heads * head_dim):
+        width = n_heads * head_dim
+        if q.dtype is not self.dtype or q.dim() < 1 or q.stride(-1) != 1:
+            raise KernelError(f"{what}: q {tuple(q.shape)} of {q.dtype} is not rows of {self.dtype_name}")
+        if T > 0 and (q_stride < width or not self._holds(q, (T - 1) * q_stride + width)):
             raise KernelError(f"{what}: rows {q_stride} apart of q {tuple(q.shape)} do not hold {T} rows of {n_heads} heads of {head_dim}")
-        if out.dim() != 2 or tuple(out.shape) != (T, n_heads * head_dim) or not out.is_contiguous():
-            raise KernelError(f"{what}: out {tuple(out.shape)} is not [{T}, {n_heads * head_dim}]")
+        if out.dtype is not self.dtype or out.shape != (T, width) or not out.is_contiguous():
+            raise KernelError(f"{what}: out {tuple(out.shape)} of {out.dtype} is not [{T}, {width}] of {self.dtype_name}")
+
+    @staticmethod
+    def _holds(t: torch.Tensor, elements: int) -> bool:
+        """Whether t's storage has so many elements from t's first on."""
+        return t.numel() >= elements or t.untyped_storage().nbytes() // t.element_size() - t.storage_offset() >= elements
 
     def kv4_attention_decode(self, q, q_stride, k_cache, v_cache, block_table, positions, seq_rows, out, token_index, partial,
                              max_chunks, n_heads, n_kv_heads, head_dim, page_size, window, scale, work) -> torch.Tensor:
