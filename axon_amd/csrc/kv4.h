@@ -79,7 +79,5 @@ __device__ __forceinline__ void kv4_pair_scale(unsigned metas, half2_t& s, half2
   c = -__builtin_bit_cast(half2_t, ((metas << 6) & 0x03C003C0u) | 0x4C004C00u) * s;
 }
 
-// One number, 32 bits.
-__device__ inline float kv4_value(unsigned n, unsigned meta) {
-  return __fmul_rn(kv4_scale_of(meta), (float)((int)n - (int)(meta & 15)));
-}
+// One of an operand's two numbers, in 32 bits.
+__device__ __forceinline__ float kv4_half(unsigned pair, int which) { return (float)__builtin_bit_cast(half2_t, pair)[which]; }

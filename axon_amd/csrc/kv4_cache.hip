@@ -24,15 +24,35 @@ __device__ inline void store8(elem_t* p, const float (&v)[8]) {
 #endif
 }
 
-// The tokens from t on that lie in one octet of slots of one request, one position behind the other: 0 if t continues such a
-// run (its first token's thread has it), or is padding (a negative position).
-__device__ inline int octet_run(const int32_t* positions, const int32_t* seq_rows, int t, int n_tokens) {
-  const int pos = positions[t], row = seq_rows[t];
-  if (pos < 0) return 0;
-  if ((pos & 7) != 0 && t > 0 && positions[t - 1] == pos - 1 && seq_rows[t - 1] == row) return 0;
-  int n = 1;
-  while (n < 8 - (pos & 7) && t + n < n_tokens && positions[t + n] == pos + n && seq_rows[t + n] == row) ++n;
-  return n;
+// Up to LIST_ROWS neighbouring tokens (or rows that are read) of a block: where each lies, and the runs that begin among them, rows that
+// lie one position behind the other in one octet of slots of one request.  A run that goes on behind them is the block's all the
+// same, and one that began before them is not: an octet's words are stored by one block, once, where a step has the whole of it.
+#define LIST_ROWS 16
+struct RowList {
+  int pos[LIST_ROWS], page[LIST_ROWS], run_first[LIST_ROWS], run_rows[LIST_ROWS], runs;
+};
+
+__device__ inline void list_rows(RowList& list, const int32_t* positions, const int32_t* seq_rows, const int32_t* block_table, int table_stride,
+                                 int first, int n, int n_tokens, int page_size) {
+  if (threadIdx.x < AXON_WAVE) {
+    const int i = threadIdx.x, t = first - 1 + i;                // lane 0: the row before them
+    const bool there = t >= 0 && t < n_tokens && i <= n + 7;
+    const int pos = there ? positions[t] : -1, row = there ? seq_rows[t] : -1;
+    if (i >= 1 && i <= n) {
+      list.pos[i - 1] = pos;
+      list.page[i - 1] = pos < 0 ? 0 : block_table[(size_t)row * table_stride + pos / page_size];        // (padding has no place)
+    }
+    const int pos_before = __shfl_up(pos, 1, AXON_WAVE), row_before = __shfl_up(row, 1, AXON_WAVE);       // (of every lane: none is left out)
+    const bool follows = i > 0 && pos >= 0 && (pos & 7) != 0 && pos_before == pos - 1 && row_before == row;
+    const uint64_t stops = __ballot(!follows), starts = stops & __ballot(i >= 1 && i <= n && pos >= 0);
+    if (starts >> i & 1) {                                       // (a run has eight rows at most: lane n + 8 follows nothing)
+      const int at = __popcll(starts & ((1ull << i) - 1));
+      list.run_first[at] = i - 1;
+      list.run_rows[at] = __builtin_ctzll(stops >> (i + 1)) + 1;
+    }
+    if (i == 0) list.runs = __popcll(starts);
+  }
+  __syncthreads();
 }
 
 // The scale word of a group of 32 dims, eight of them in each of four neighbouring lanes, and the lane's eight numbers.
@@ -58,9 +78,17 @@ __device__ inline unsigned kv4_quantise8(const float (&x)[8], unsigned (&n)[8]) 
     for (int i = 0; i < 8; ++i) n[i] = 0;
     return bad ? KV4_NAN : 0;
   }
-  const float z = fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.0f), 15.0f);
+  // x / s, correctly rounded, by the scale's reciprocal and what the product leaves: q = x r is within two units of its last place, the rest
+  // x - q s is exact, and q + rest r is off by 2^-23 units before it is rounded, while a quotient by a scale of six bits
+  // is 2^-7 units or more away from the middle between two numbers, where the rounding would turn.
+  const float r = __fdiv_rn(1.0f, s);
+  auto quotient = [&](float v) {
+    const float q = __fmul_rn(v, r);
+    return __builtin_fmaf(__builtin_fmaf(-q, s, v), r, q);
+  };
+  const float z = fminf(fmaxf(rintf(quotient(-lo)), 0.0f), 15.0f);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) n[i] = (unsigned)fminf(fmaxf(__fadd_rn(rintf(__fdiv_rn(x[i], s)), z), 0.0f), 15.0f);
+  for (int i = 0; i < 8; ++i) n[i] = (unsigned)fminf(fmaxf(__fadd_rn(rintf(quotient(x[i])), z), 0.0f), 15.0f);
   return bits | (unsigned)z;
 }
 
@@ -80,94 +108,130 @@ __device__ inline void rotated8(const elem_t* head, const float* tab, int c0, in
   }
 }
 
-// A block a token: its queries (a thread the eight pairs of dims i .. i + 7 and i + half .., or eight dims behind the rotated
-// ones), its keys (a thread a word) and, at the first token of an octet of slots, the values of all tokens of the octet that
-// the step brings (a thread eight dims of up to eight positions).
+// The blocks behind the first kv_blocks have the queries of Q_TOKENS tokens each: a thread the eight pairs of dims i .. i + 7 and i + half .. (or
+// sixteen dims behind the rotated ones) of several heads of a token, whose sines and cosines it reads once.  The first, which take longer, have the keys and
+// values of up to `rows` tokens: a thread a word of keys, or eight dims of a run's values, whose words hold up to eight positions.
+// Bound by its bytes in prompts (qkv in, q and the cache out: 8192 tokens of 28 and 4 heads of 128 dims take 31 us, 139 MB at 4.5 TB/s), by its waits
+// in steps of few tokens (8: 5.4 us; of which a launch that does nothing is 2.9).
+template <int Q_TOKENS>
 __global__ void __launch_bounds__(256)
 rope_kv4_write_kernel(const elem_t* qkv, long qkv_stride, elem_t* q_out, long q_stride, const float* __restrict__ table,
                       const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows,
                       const int32_t* __restrict__ block_table, int table_stride, unsigned char* __restrict__ k_cache,
                       unsigned char* __restrict__ v_cache, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rotary_dim,
-                      int page_size, int write_kv) {
-  const int t = blockIdx.x, half = rotary_dim / 2;
-  const elem_t* row = qkv + (size_t)t * qkv_stride;
-  const float* tab = table + (size_t)t * half * 2;
-  const int q_units = half / 8 + (head_dim - rotary_dim) / 8;
-  for (int u = threadIdx.x; u < n_heads * q_units; u += 256) {
-    const int head = u / q_units, c = u % q_units;
-    const elem_t* src = row + head * head_dim;
-    elem_t* dst = q_out + (size_t)t * q_stride + head * head_dim;
-    if (c < half / 8) {
-      float a[8], b[8];
-      load8(src + 8 * c, a);
-      load8(src + half + 8 * c, b);
+                      int page_size, int kv_blocks, int rows) {
+  __shared__ RowList list;
+  const int half = rotary_dim / 2;
+  if ((int)blockIdx.x >= kv_blocks) {
+    const int units = head_dim / 16, lanes = 256 / units / Q_TOKENS;           // lanes that share a token's heads
+    const int c = threadIdx.x % units, slot = threadIdx.x / units, t = (blockIdx.x - kv_blocks) * Q_TOKENS + slot / lanes;
+    if (t >= n_tokens) return;
+    const bool turn = c < half / 8;
+    const int d0 = turn ? 8 * c : rotary_dim + 16 * (c - half / 8), d1 = turn ? d0 + half : d0 + 8;
+    float sin_cos[16];
+    if (turn) {
+      const float4* tab = reinterpret_cast<const float4*>(table + ((size_t)t * half + d0) * 2);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float s = tab[2 * (8 * c + i)], co = tab[2 * (8 * c + i) + 1], x = a[i];
-        a[i] = __fsub_rn(__fmul_rn(x, co), __fmul_rn(b[i], s));
-        b[i] = __fadd_rn(__fmul_rn(x, s), __fmul_rn(b[i], co));
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = tab[i];
+        sin_cos[4 * i] = v.x; sin_cos[4 * i + 1] = v.y; sin_cos[4 * i + 2] = v.z; sin_cos[4 * i + 3] = v.w;
       }
-      store8(dst + 8 * c, a);
-      store8(dst + half + 8 * c, b);
-    } else {
-      float a[8];
-      const int d = rotary_dim + 8 * (c - half / 8);
-      load8(src + d, a);
-      store8(dst + d, a);
     }
-  }
-  if (!write_kv) return;
-  const int pos = positions[t];
-  if (pos < 0) return;                                       // padding
-  const int words = head_dim / 8, kv_units = n_kv_heads * words;
-  const size_t head_bytes = (size_t)page_size * kv4_row_bytes(head_dim);
-  const int page = block_table[(size_t)seq_rows[t] * table_stride + pos / page_size], slot = pos % page_size;
-  const int run = octet_run(positions, seq_rows, t, n_tokens);
-  for (int u = threadIdx.x; u < 2 * kv_units; u += 256) {      // (a group's four lanes are in it together: words come in fours)
-    const bool is_v = u >= kv_units;
-    if (is_v && run == 0) break;
-    const int w = is_v ? u - kv_units : u, kvh = w / words, c0 = w % words * 8;
-    if (!is_v) {
-      float x[8];
-      unsigned n[8];
-      rotated8(row + (n_heads + kvh) * head_dim, tab, c0, rotary_dim, x);
-      const unsigned meta = kv4_quantise8(x, n);
-      unsigned word = 0;
+    const elem_t* src = qkv + (size_t)t * qkv_stride;
+    elem_t* dst = q_out + (size_t)t * q_stride;
+    constexpr int AHEAD = AXON_BF16 ? 4 : 2;                   // heads asked for before the first is stored (the rows may be the same)
+    for (int head = slot % lanes; head < n_heads; head += AHEAD * lanes) {
+      float a[AHEAD][8], b[AHEAD][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) word |= __builtin_rotateleft32(n[i], kv4_place(i));
-      unsigned char* base = k_cache + ((size_t)page * n_kv_heads + kvh) * head_bytes;
-      reinterpret_cast<unsigned*>(base)[slot * words + c0 / 8] = word;
-      if (c0 % 32 == 0)
-        reinterpret_cast<uint16_t*>(base + page_size * head_dim / 2)[slot * (head_dim / 32) + c0 / 32] = (uint16_t)meta;
-      continue;
+      for (int n = 0; n < AHEAD; ++n) {
+        const int at = min(head + n * lanes, n_heads - 1) * head_dim;
+        load8(src + at + d0, a[n]);
+        load8(src + at + d1, b[n]);
+      }
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        if (head + n * lanes >= n_heads) break;
+        if (turn)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float s = sin_cos[2 * i], co = sin_cos[2 * i + 1], x = a[n][i];
+            a[n][i] = __fsub_rn(__fmul_rn(x, co), __fmul_rn(b[n][i], s));
+            b[n][i] = __fadd_rn(__fmul_rn(x, s), __fmul_rn(b[n][i], co));
+          }
+        const int at = (head + n * lanes) * head_dim;
+        store8(dst + at + d0, a[n]);
+        store8(dst + at + d1, b[n]);
+      }
     }
-    unsigned char* base = v_cache + ((size_t)page * n_kv_heads + kvh) * head_bytes;
+    return;
+  }
+  const int first = blockIdx.x * rows, n = min(rows, n_tokens - first), words = head_dim / 8, kv_units = n_kv_heads * words, slots = page_size - 1;
+  const size_t head_bytes = (size_t)page_size * kv4_row_bytes(head_dim);
+  // keys: token i, word w of its keys; values: the same, of a run's first token (units come in fours, a group's lanes, and so do threads)
+  auto keys = [&](int i, int w, float(&x)[8]) {
+    rotated8(qkv + (size_t)(first + i) * qkv_stride + (n_heads + w / words) * head_dim, table + (size_t)(first + i) * half * 2, w % words * 8,
+             rotary_dim, x);
+  };
+  auto values = [&](int i, int w, float(&x)[8]) {
+    load8(qkv + (size_t)(first + i) * qkv_stride + (n_heads + n_kv_heads) * head_dim + w * 8, x);
+  };
+  // a thread's first unit is asked for before anything is known of the tokens' places
+  float ahead[8];
+  bool fresh = true;
+  int u = threadIdx.x;
+  if (u < n * kv_units) keys(u / kv_units, u % kv_units, ahead);
+  else if (u < (n + 1) * kv_units) values(0, u - n * kv_units, ahead);
+  list_rows(list, positions, seq_rows, block_table, table_stride, first, n, n_tokens, page_size);
+  for (; u < n * kv_units; u += 256, fresh = false) {
+    const int i = u / kv_units, w = u % kv_units, kvh = w / words, c0 = w % words * 8, pos = list.pos[i];
+    if (!fresh) keys(i, w, ahead);
+    if (pos < 0) continue;
+    unsigned numbers[8];
+    const unsigned meta = kv4_quantise8(ahead, numbers);
+    unsigned word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) word |= __builtin_rotateleft32(numbers[e], kv4_place(e));
+    unsigned char* base = k_cache + ((size_t)list.page[i] * n_kv_heads + kvh) * head_bytes;
+    const int slot = pos & slots;
+    reinterpret_cast<unsigned*>(base)[slot * words + c0 / 8] = word;
+    if (c0 % 32 == 0) reinterpret_cast<uint16_t*>(base + page_size * head_dim / 2)[slot * (head_dim / 32) + c0 / 32] = (uint16_t)meta;
+  }
+  for (u -= n * kv_units; u < list.runs * kv_units; u += 256, fresh = false) {
+    const int run = u / kv_units, w = u % kv_units, kvh = w / words, c0 = w % words * 8, i0 = list.run_first[run], run_rows = list.run_rows[run];
+    const int slot = list.pos[i0] & slots;
+    unsigned char* base = v_cache + ((size_t)list.page[i0] * n_kv_heads + kvh) * head_bytes;
     uint16_t* scales = reinterpret_cast<uint16_t*>(base + page_size * head_dim / 2) + ((slot / 8) * (head_dim / 32) + c0 / 32) * 8;
     unsigned word[8], mask = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) word[i] = 0;
-    for (int j = 0; j < run; ++j) {
-      float x[8];
-      unsigned n[8];
-      load8(row + (size_t)j * qkv_stride + (n_heads + n_kv_heads + kvh) * head_dim + c0, x);
-      const unsigned meta = kv4_quantise8(x, n);
-      const int e = (slot & 7) + j, at = kv4_place(e);
-      auto turned = [&](unsigned v) { return __builtin_rotateleft32(v, at); };
-      mask |= turned(15u);
+    for (int e = 0; e < 8; ++e) word[e] = 0;
+    auto take = [&](int e, const float(&x)[8]) {
+      unsigned numbers[8];
+      const unsigned meta = kv4_quantise8(x, numbers);
+      const int at = kv4_place(e);
+      mask |= __builtin_rotateleft32(15u, at);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) word[i] |= turned(n[i]);
+      for (int d = 0; d < 8; ++d) word[d] |= __builtin_rotateleft32(numbers[d], at);
       if (c0 % 32 == 0) scales[e] = (uint16_t)meta;
-    }
+    };
     unsigned* dst = reinterpret_cast<unsigned*>(base) + (slot / 8) * head_dim + c0;
-    if (run == 8) {
+    if (run_rows == 8) {
+      float x[8][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) values(i0 + e, w, x[e]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) take(e, x[e]);
       reinterpret_cast<uint4*>(dst)[0] = make_uint4(word[0], word[1], word[2], word[3]);
       reinterpret_cast<uint4*>(dst)[1] = make_uint4(word[4], word[5], word[6], word[7]);
     } else {
-      // a part of the octet: its own bits alone, so that runs of one octet that lie apart in a step do not undo each other
+      for (int e = 0; e < run_rows; ++e) {
+        if (e > 0 || i0 > 0 || !fresh) values(i0 + e, w, ahead); // (the first token's: asked for already)
+        take((slot & 7) + e, ahead);
+      }
+      // a part of the octet: its own bits alone, so that the octet's other runs, which may lie elsewhere in the step, are not undone
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        __hip_atomic_fetch_and(dst + i, ~mask, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_fetch_or(dst + i, word[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (int d = 0; d < 8; ++d) {
+        __hip_atomic_fetch_and(dst + d, ~mask, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_fetch_or(dst + d, word[d], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
   }
@@ -189,60 +253,88 @@ extern "C" int axk_rope_kv4_write(const void* qkv, long qkv_stride, void* q_out,
                   q_stride * sizeof(elem_t) % 16 == 0,
               "rope_kv4_write: rows must be 16-byte aligned (strides %ld and %ld)", qkv_stride, q_stride);
   AXK_REQUIRE(!write_kv || ((uintptr_t)k_cache % 16 == 0 && (uintptr_t)v_cache % 16 == 0), "rope_kv4_write: caches must be 16-byte aligned");
+  AXK_REQUIRE((uintptr_t)table % 16 == 0, "rope_kv4_write: the table must be 16-byte aligned");
   if (n_tokens == 0) return 0;
-  rope_kv4_write_kernel<<<n_tokens, 256, 0, (hipStream_t)stream>>>(
-      (const elem_t*)qkv, qkv_stride, (elem_t*)q_out, q_stride, table, positions, seq_rows, block_table, table_stride,
-      (unsigned char*)k_cache, (unsigned char*)v_cache, n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, page_size, write_kv);
+  // Few tokens: a block each for its queries and for its keys and values.  Of 28 query and 4 key/value heads of 128 dims, so or in blocks of four
+  // and eight tokens: 8 single tokens 5.2 and 10.6 us, 128 8.7 and 13.7, 256 12.0 and 17.3; a portion of 64 tokens 7.8 and 10.0, of 256
+  // 8.4 and 10.3, of 512 9.6 and 10.6.  (Blocks of sixteen tokens take 33 us for 8192, of eight 31.)
+  const bool few = n_tokens <= 512;
+  const int rows = few ? 1 : 8, q_blocks = few ? n_tokens : ceil_div(n_tokens, 4), kv_blocks = write_kv ? ceil_div(n_tokens, rows) : 0;
+  const unsigned blocks = q_blocks + kv_blocks;
+#define LAUNCH(Q_TOKENS)                                                                                                          \
+  rope_kv4_write_kernel<Q_TOKENS><<<blocks, 256, 0, (hipStream_t)stream>>>(                                                       \
+      (const elem_t*)qkv, qkv_stride, (elem_t*)q_out, q_stride, table, positions, seq_rows, block_table, table_stride,            \
+      (unsigned char*)k_cache, (unsigned char*)v_cache, n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, page_size, kv_blocks, rows)
+  if (few) LAUNCH(1);
+  else LAUNCH(4);
+#undef LAUNCH
   AXK_LAUNCH_CHECK("rope_kv4_write");
   return 0;
 }
 
 // Rows (seq_rows[i], positions[i]) of the cache as plain rows [n][kv heads][head_dim] of the compute dtype, each number rounded
-// once (bfloat16 holds eight of its up to ten bits).  A thread has eight dims: of a key's row one word, of the values the eight
-// words that hold them for all rows of an octet that lie side by side in the list.
+// once (bfloat16 holds eight of its up to ten bits).  grid (lists of LIST_ROWS rows, keys | values): a thread a word of keys, or the words of
+// eight dims of a run's values, which it unpacks as the products' operands are.  A run of whole octets is its
+// first block's; no words are read twice.  Bound by the rows that it stores: eight requests' 16384 positions of 4 heads of 128 dims take 80 us, 344 MB at 4.3 TB/s;
+// by its waits for few (301 rows: 4.7 us).
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
                 const int32_t* __restrict__ block_table, int table_stride, const int32_t* __restrict__ positions,
                 const int32_t* __restrict__ seq_rows, elem_t* __restrict__ k_out, elem_t* __restrict__ v_out, int n_rows,
                 int n_kv_heads, int head_dim, int page_size) {
-  const int words = head_dim / 8, kv_units = n_kv_heads * words;
-  const long at = (long)blockIdx.x * 256 + threadIdx.x;
-  const int r = (int)(at / (2 * kv_units)), u = (int)(at % (2 * kv_units));
-  if (r >= n_rows) return;
-  const bool is_v = u >= kv_units;
-  const int w = is_v ? u - kv_units : u, kvh = w / words, c0 = w % words * 8;
-  const int pos = positions[r];
-  const size_t out_row = (size_t)n_kv_heads * head_dim;
-  elem_t* dst = (is_v ? v_out : k_out) + (size_t)r * out_row + kvh * head_dim + c0;
-  float v[8];
-  if (pos < 0) {                                             // padding: a row of zeros
+  __shared__ RowList list;
+  const int first = blockIdx.x * LIST_ROWS, n = min(LIST_ROWS, n_rows - first);
+  list_rows(list, positions, seq_rows, block_table, table_stride, first, n, n_rows, page_size);
+  const int words = head_dim / 8, kv_units = n_kv_heads * words, slots = page_size - 1;
+  const size_t out_row = (size_t)n_kv_heads * head_dim, head_bytes = (size_t)page_size * kv4_row_bytes(head_dim);
+  const Kv4Masks masks = kv4_masks();
+  if (blockIdx.y == 0) {
+    for (int u = threadIdx.x; u < n * kv_units; u += 256) {
+      const int i = u / kv_units, w = u % kv_units, kvh = w / words, c0 = w % words * 8, pos = list.pos[i], slot = pos & slots;
+      float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};               // (padding)
+      if (pos >= 0) {
+        const unsigned char* base = k_cache + ((size_t)list.page[i] * n_kv_heads + kvh) * head_bytes;
+        const unsigned word = reinterpret_cast<const unsigned*>(base)[slot * words + c0 / 8];
+        const unsigned meta = reinterpret_cast<const uint16_t*>(base + page_size * head_dim / 2)[slot * (head_dim / 32) + c0 / 32];
+        half2_t sc[4], cc[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    store8(dst, v);
+        for (int e = 0; e < 4; ++e) kv4_pair_scale(meta | meta << 16, sc[e], cc[e]);
+        const u32x4 pairs = kv4_operand(word, sc, cc, masks);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = kv4_half(pairs[e / 2], e % 2);
+      }
+      store8(k_out + (size_t)(first + i) * out_row + kvh * head_dim + c0, v);
+    }
     return;
   }
-  const int run = is_v ? octet_run(positions, seq_rows, r, n_rows) : 1;
-  if (run == 0) return;
-  const int page = block_table[(size_t)seq_rows[r] * table_stride + pos / page_size], slot = pos % page_size;
-  const unsigned char* base = (is_v ? v_cache : k_cache) + ((size_t)page * n_kv_heads + kvh) * page_size * kv4_row_bytes(head_dim);
-  const uint16_t* scales = reinterpret_cast<const uint16_t*>(base + page_size * head_dim / 2);
-  if (!is_v) {
-    const unsigned word = reinterpret_cast<const unsigned*>(base)[slot * words + c0 / 8];
-    const unsigned meta = scales[slot * (head_dim / 32) + c0 / 32];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = kv4_value(__builtin_rotateright32(word, kv4_place(i)) & 15u, meta);
-    store8(dst, v);
-    return;
+  for (int u = threadIdx.x; u < n * kv_units; u += 256) {                          // padding's values
+    const int i = u / kv_units, w = u % kv_units;
+    const float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (list.pos[i] < 0) store8(v_out + (size_t)(first + i) * out_row + w * 8, v);
   }
-  const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned*>(base) + (slot / 8) * head_dim + c0);
-  const uint4 w0 = src[0], w1 = src[1];
-  const unsigned word[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-  for (int j = 0; j < run; ++j) {
-    const int e = (slot & 7) + j;
-    const unsigned meta = scales[((slot / 8) * (head_dim / 32) + c0 / 32) * 8 + e];
+  for (int u = threadIdx.x; u < list.runs * kv_units; u += 256) {
+    const int run = u / kv_units, w = u % kv_units, kvh = w / words, c0 = w % words * 8, i0 = list.run_first[run];
+    const int slot = list.pos[i0] & slots, low = slot & 7, high = low + list.run_rows[run];
+    const unsigned char* base = v_cache + ((size_t)list.page[i0] * n_kv_heads + kvh) * head_bytes;
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned*>(base) + (slot / 8) * head_dim + c0);
+    const uint4 metas = *reinterpret_cast<const uint4*>(base + page_size * head_dim / 2 + ((slot / 8) * (head_dim / 32) + c0 / 32) * 16);
+    const uint4 w0 = src[0], w1 = src[1];
+    const unsigned word[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w}, meta[4] = {metas.x, metas.y, metas.z, metas.w};
+    half2_t sc[4], cc[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = kv4_value(__builtin_rotateright32(word[i], kv4_place(e)) & 15u, meta);
-    store8(dst + j * out_row, v);
+    for (int e = 0; e < 4; ++e) kv4_pair_scale(meta[e], sc[e], cc[e]);
+    u32x4 pairs[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) pairs[d] = kv4_operand(word[d], sc, cc, masks);
+    elem_t* dst = v_out + (size_t)(first + i0) * out_row + kvh * head_dim + c0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e < low || e >= high) continue;
+      float v[8];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) v[d] = kv4_half(pairs[d][e / 2], e % 2);
+      store8(dst + (size_t)(e - low) * out_row, v);
+    }
   }
 }
 
@@ -253,10 +345,8 @@ extern "C" int axk_kv4_read(const void* k_cache, const void* v_cache, const int3
               "kv4_read: n=%d nkv=%d head_dim %d page size %d are not taken", n_rows, n_kv_heads, head_dim, page_size);
   AXK_REQUIRE((uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0 && (uintptr_t)k_cache % 16 == 0 && (uintptr_t)v_cache % 16 == 0,
               "kv4_read: caches and rows must be 16-byte aligned");
-  const long units = (long)n_rows * 2 * n_kv_heads * (head_dim / 8);
-  AXK_REQUIRE(units / 256 < (1l << 31) - 1, "kv4_read: %d rows are too many", n_rows);
   if (n_rows == 0) return 0;
-  kv4_read_kernel<<<(unsigned)((units + 255) / 256), 256, 0, (hipStream_t)stream>>>(
+  kv4_read_kernel<<<dim3(ceil_div(n_rows, LIST_ROWS), 2), 256, 0, (hipStream_t)stream>>>(
       (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride, positions, seq_rows, (elem_t*)k_out,
       (elem_t*)v_out, n_rows, n_kv_heads, head_dim, page_size);
   AXK_LAUNCH_CHECK("kv4_read");
