@@ -516,7 +516,8 @@ int axk_kv4_ok(int head_dim, int page_size);
 int axk_kv4_row_bytes(int head_dim);
 // Rotate-half on the first rotary_dim dims (a multiple of 16) of each q and k head of qkv [T][(nh + 2 nkv) hd], rows qkv_stride
 // apart: q to q_out (rows q_stride apart; qkv's own q columns are allowed), k and v quantised into the pages at each token's
-// position.  write_kv = 0: q alone, of rows that hold nh heads.  Slots of other positions are left as they were.
+// position (a position of a request once in a step).  write_kv = 0: q alone, of rows that hold nh heads.  Slots of other positions are
+// left as they were.
 int axk_rope_kv4_write(const void* qkv, long qkv_stride, void* q_out, long q_stride, const float* table, const int32_t* positions,
                        const int32_t* seq_rows, const int32_t* block_table, int table_stride, void* k_cache, void* v_cache,
                        int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rotary_dim, int page_size, int write_kv,

@@ -979,8 +979,8 @@ extern "C" int axk_kv4_attention_decode(const void* q, int q_stride, const void*
   AXK_REQUIRE(max_chunks >= 1 && max_chunks <= KV4_ITEM_FACTOR, "kv4_attention_decode: %d chunks of a token (at most %d)", max_chunks,
               KV4_ITEM_FACTOR);
   AXK_REQUIRE(n_work >= 0 && (n_work == 0 || work != nullptr), "kv4_attention_decode: a work list of %d items", n_work);
-  AXK_REQUIRE(partial != nullptr && (uintptr_t)partial % 16 == 0, "kv4_attention_decode: needs its workspace, 16-byte aligned");
   if (n_tokens == 0 || n_work == 0) return 0;
+  AXK_REQUIRE(partial != nullptr && (uintptr_t)partial % 16 == 0, "kv4_attention_decode: needs its workspace, 16-byte aligned");
   const dim3 units(n_kv_heads * sets, n_work < 65535 ? n_work : 65535, (n_work + 65534) / 65535);
 #define LAUNCH(HD)                                                                                                              \
   {                                                                                                                             \
@@ -1030,16 +1030,17 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
 #define LAUNCH(HD, HPB)                                                                                                         \
   {                                                                                                                             \
     constexpr int lds = Kv4Stage<HD>::ALL;                                                                                      \
-    static bool configured = false;                                                                                             \
-    if (!configured) {                                                                                                          \
-      hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<HD, HPB>),                           \
-                                         hipFuncAttributeMaxDynamicSharedMemorySize, lds);                                      \
-      if (e != hipSuccess) {                                                                                                    \
-        axk_set_error("kv4_attention_prefill: cannot reserve %d bytes of LDS: %s", lds, hipGetErrorString(e));                  \
-        return -2;                                                                                                              \
-      }                                                                                                                         \
-      configured = true;                                                                                                        \
+    static uint64_t configured = 0;                                                            /* a bit for each device */      \
+    int device = 0;                                                                                                             \
+    hipError_t e = hipGetDevice(&device);                                                                                       \
+    if (e == hipSuccess && !(configured >> (device & 63) & 1))                                                                  \
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(&kv4_prefill_kernel<HD, HPB>),                                      \
+                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);                                                 \
+    if (e != hipSuccess) {                                                                                                      \
+      axk_set_error("kv4_attention_prefill: cannot reserve %d bytes of LDS: %s", lds, hipGetErrorString(e));                    \
+      return -2;                                                                                                                \
     }                                                                                                                           \
+    configured |= 1ull << (device & 63);                                                                                        \
     kv4_prefill_kernel<HD, HPB><<<dim3(n_kv_heads * ((group + HPB - 1) / HPB), n_tiles), 256 * HPB, lds, (hipStream_t)stream>>>( \
         (const elem_t*)q, q_stride, (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride,    \
         positions, seq_rows, (elem_t*)out, tiles, partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);             \

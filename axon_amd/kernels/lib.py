@@ -1717,7 +1717,8 @@ class Kernels:
                        rotary_dim, page_size, write_kv=True) -> None:
         """`rope_kv_write` for a cache held in 4 bits: rotate-half on the first `rotary_dim` dims (a multiple of 16) of every q and
         k head of qkv [T, (n_heads + 2 n_kv_heads) head_dim], whose rows may lie apart; q to q_out [T, n_heads head_dim] (qkv's own
-        columns are allowed), k and v quantised from 32 bits into the pages.  Without write_kv, q alone."""
+        columns are allowed), k and v quantised from 32 bits into the pages; a request's position is there once in a step (of two that are
+        the same neither may be what is held).  Without write_kv, q alone."""
         self._elem(qkv, "rope qkv"); self._elem(q_out, "rope q"); self._f32(table, "rope table")
         T = self._kv4_step("rope_kv4_write", k_cache if write_kv else None, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim,
                            page_size, qkv, q_out, table)
