@@ -315,6 +315,8 @@ def main() -> int:
     ap.add_argument("--dtype", default="bfloat16")
     ap.add_argument("--page-size", type=int, default=16, help="positions in a cache page (default: the 16 that the "
                     "measured configurations name; the engine's own default is 64, a block of its attention kernels)")
+    ap.add_argument("--cache-bits", type=int, default=0, choices=[0, 4], help="4: keys and values held in 4 bits (default: in the compute "
+                    "dtype)")
     ap.add_argument("--sizes", default="7b", choices=sorted(SIZES), help="layer sizes of Qwen2.5-7B (the default), 14B or 32B")
     ap.add_argument("--no-points", action="store_true", help="only the headline batch and the prefill point")
     ap.add_argument("--phase", default="all", choices=["all", "prefill", "decode", "mixed", "bandwidth"],
@@ -357,7 +359,8 @@ def main() -> int:
     # the largest size takes its pool from the memory that is free (context 16,384 for up to 64 requests)
     num_pages = 0 if args.sizes == "32b" else -(-tokens_needed // page) + most_batch
     llm = axon_amd.load(cfg, dtype=args.dtype, random_seed=0, init_std=0.02, page_size=page, num_pages=num_pages,
-                        max_seqs=most_batch, max_batch_tokens=max(prompt_len, 2048), max_seq_len=ctx_len)
+                        max_seqs=most_batch, max_batch_tokens=max(prompt_len, 2048), max_seq_len=ctx_len,
+                        cache_bits=args.cache_bits)
     eng = llm.engine
     gen = torch.Generator().manual_seed(0)
 
@@ -434,7 +437,7 @@ def main() -> int:
         mid_ctx = prompt_len + 1 + warmup + n_steps / 2
         for rid in ids:
             eng.release(rid)
-        kv_bytes = batch * mid_ctx * L * 2 * nkv * hd * elem
+        kv_bytes = batch * mid_ctx * L * 2 * nkv * (hd // 2 + hd // 16 if args.cache_bits else hd * elem)
         step_s = dt / n_steps
         return {"tok_s": batch * n_steps / dt, "ms": step_s * 1e3,
                 "frac": (weight_bytes + kv_bytes) / step_s / HBM_BYTES_PER_S, "bytes": weight_bytes + kv_bytes}
@@ -544,7 +547,7 @@ def main() -> int:
         "config": {"model": name, "layers": L, "layers_of_config": full_layers, "hidden": dim,
                    "heads": nh, "kv_heads": nkv, "head_dim": hd, "intermediate": ffn, "vocab": V, "batch": args.batch,
                    "global_batch": args.batch, "seq_len": prompt_len, "generated": steps, "context": ctx_len,
-                   "page_size": page, "cache_pages": cache_pages, "parallelism": "single GPU",
+                   **({"cache_bits": args.cache_bits} if args.cache_bits else {}), "page_size": page, "cache_pages": cache_pages, "parallelism": "single GPU",
                    "graphs": graphs_on, "batch_invariant": True},
         "prefill": prefill_point,
         "roofline": {"bound": "hbm", "achieved": round(achieved, 1), "peak": HBM_BYTES_PER_S / 1e9, "unit": "GB/s",
