@@ -165,6 +165,7 @@ def decode_scratch_floats(k, window: int, n_heads: int, head_dim: int, max_seqs:
     return k.attention_decode_workspace(max_seqs, n_heads, head_dim, 1 << (most - 1).bit_length())
 
 
+NORMED_ROWS = 16        # the most rows that a product takes with the norm of its operand inside (`gemm_normed_ok`)
 KV4_SINGLES = 16        # portions of up to so many tokens go token by token to the 4-bit cache's kernel for single tokens
 
 
@@ -222,6 +223,7 @@ class GQAttention(Mixer):
         self.n = {k: base + names.get(k, k + "_proj") for k in ("q", "k", "v", "o")}
         self.w_qkv = self.b_qkv = self.w_o = self.b_o = None
         self.cache_bits = 0                  # 0: in the compute dtype
+        self.unturned = None
         self._max_context = None
         self._kernels = None                 # those that want a workspace in decoding steps
         self.decode_chunk = 1 << 30          # until `load` has asked the kernels: one chunk
@@ -307,6 +309,8 @@ class GQAttention(Mixer):
             if not rt.k.kv4_ok(self.hd, 64) or self.cache_spec().head_dim != rt.k.kv4_row_bytes(self.hd):
                 raise ConfigError(f"{self.prefix}: the 4-bit cache's kernels do not take heads of {self.hd}")
             self._kernels, self._work_list, self._max_context = rt.k, rt.k.kv4_decode_work, rt.k.kv4_max_context
+            # sines and cosines of no angle for the rows that the product with the norm inside takes
+            self.unturned = torch.tensor([0.0, 1.0], device=rt.device).repeat(NORMED_ROWS, self.hd // 2, 1)
         self.w_qkv = rt.k.prepare_weight(store.fused_matrix([self.n[k] + ".weight" for k in ("q", "k", "v")]))
         biases = [store.vector(self.n[k] + ".bias", optional=True) for k in ("q", "k", "v")] if self.qkv_bias else []
         present = [b is not None for b in biases]
@@ -328,8 +332,9 @@ class GQAttention(Mixer):
     def applies_preceding_norm(self, ctx) -> bool:
         k = ctx.rt.k
         rows = self.q_dim + 2 * self.kv_dim
-        return (isinstance(self.w_qkv, PackedMatrix) and self.position is not None and not self.cache_bits
-                and k.gemm_qkv_rope_ok(ctx.n_tokens, rows, self.hidden, self.hd, self.position.rotary_dim)
+        rotary = self.hd if self.cache_bits else self.position.rotary_dim if self.position is not None else 0
+        return (isinstance(self.w_qkv, PackedMatrix) and rotary > 0
+                and k.gemm_qkv_rope_ok(ctx.n_tokens, rows, self.hidden, self.hd, rotary)
                 and k.gemm_normed_ok(ctx.n_tokens, rows, self.hidden))
 
     def forward(self, ctx, binding: CacheBinding, h, residual, following=None) -> None:
@@ -386,12 +391,20 @@ class GQAttention(Mixer):
 
     def _forward_kv4(self, ctx, group, k_cache, v_cache, writes, h, residual, following) -> None:
         k, T = ctx.rt.k, h.shape[0]
-        if isinstance(h, PrecedingNorm):
-            h = h.apply(ctx)
         table, rotary = (self.position.tables(ctx), self.position.rotary_dim) if self.position is not None else (ctx.no_rotation(), 0)
         width = self.q_dim + (2 * self.kv_dim if writes else 0)
         qkv = ctx.ws.take((T, width), ctx.rt.dtype)
-        k.gemm(h, self.w_qkv[:width], qkv, None if self.b_qkv is None else self.b_qkv[:width], MODE_STORE)
+        w, bias = self.w_qkv[:width], None if self.b_qkv is None else self.b_qkv[:width]
+        if isinstance(h, PrecedingNorm) and not (k.gemm_normed_ok(T, width, self.hidden, gain=h.gain)
+                                                 and k.gemm_qkv_rope_ok(T, width, self.hidden, self.hd, self.hd)):
+            h = h.apply(ctx)
+        if isinstance(h, PrecedingNorm):
+            # Few rows: the norm and the product in one launch, every head a query's that turns by an angle of zero (x 1 - y 0 is x).  The
+            # rotation is the next kernel's, which quantises keys that were not rounded behind it.
+            k.gemm_normed_qkv_rope(h.rows, h.gain, h.eps, w, bias, qkv, self.unturned[:T], ctx.positions, ctx.seq_rows, group.block_table,
+                                   None, None, width // self.hd, self.nkv, self.hd, group.page_size, False)
+        else:
+            k.gemm(h, w, qkv, bias, MODE_STORE)
         q = qkv[:, :self.q_dim]
         sizes = (self.nh, self.nkv, self.hd)
         k.rope_kv4_write(qkv, q, table, ctx.positions, ctx.seq_rows, group.block_table, k_cache, v_cache, *sizes, rotary,
