@@ -92,27 +92,32 @@ __device__ inline unsigned kv4_quantise8(const float (&x)[8], unsigned (&n)[8]) 
   return bits | (unsigned)z;
 }
 
-// Dims c0 .. c0 + 7 of a head's row behind the rotation (rotate-half on the first rotary_dim dims; half a multiple of 8).
+// Dims c0 .. c0 + 7 of a head's row behind the rotation (rotate-half on the first rotary_dim dims; half a multiple of 8).  All loads are without a
+// branch, so that they are under way together: dims that do not turn read themselves and the table's first 64 bytes, which have to be
+// there also where nothing turns.
 __device__ inline void rotated8(const elem_t* head, const float* tab, int c0, int rotary_dim, float (&out)[8]) {
-  load8(head + c0, out);
-  if (c0 >= rotary_dim) return;
-  const int half = rotary_dim / 2;
-  const bool upper = c0 >= half;
-  const int i0 = upper ? c0 - half : c0;
-  float other[8];
-  load8(head + (upper ? c0 - half : c0 + half), other);
+  const int half = rotary_dim / 2, to = c0 >= half ? -half : half;
+  const bool turn = c0 < rotary_dim, upper = c0 >= half;
+  const float4* at = reinterpret_cast<const float4*>(tab + (turn ? 2 * min(c0, c0 + to) : 0));
+  float x[8], y[8];
+  float4 sin_cos[4];
+  load8(head + c0, x);
+  load8(head + (c0 + (turn ? to : 0)), y);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sin_cos[i] = at[i];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float s = tab[2 * (i0 + i)], c = tab[2 * (i0 + i) + 1];
-    out[i] = upper ? __fadd_rn(__fmul_rn(other[i], s), __fmul_rn(out[i], c)) : __fsub_rn(__fmul_rn(out[i], c), __fmul_rn(other[i], s));
+    const float s = i % 2 ? sin_cos[i / 2].z : sin_cos[i / 2].x, c = i % 2 ? sin_cos[i / 2].w : sin_cos[i / 2].y;
+    const float turned = upper ? __fadd_rn(__fmul_rn(y[i], s), __fmul_rn(x[i], c)) : __fsub_rn(__fmul_rn(x[i], c), __fmul_rn(y[i], s));
+    out[i] = turn ? turned : x[i];
   }
 }
 
 // The blocks behind the first kv_blocks have the queries of Q_TOKENS tokens each: a thread the eight pairs of dims i .. i + 7 and i + half .. (or
 // sixteen dims behind the rotated ones) of several heads of a token, whose sines and cosines it reads once.  The first, which take longer, have the keys and
 // values of up to `rows` tokens: a thread a word of keys, or eight dims of a run's values, whose words hold up to eight positions.
-// Bound by its bytes in prompts (qkv in, q and the cache out: 8192 tokens of 28 and 4 heads of 128 dims take 31 us, 139 MB at 4.5 TB/s), by its waits
-// in steps of few tokens (8: 5.4 us; of which a launch that does nothing is 2.9).
+// Bound by its bytes in prompts (qkv in, q and the cache out: 8192 tokens of 28 and 4 heads of 128 dims take 25 us, 143 MB at 5.7 TB/s), by its waits
+// in steps of few tokens (8: 4.8 us; a launch of the queries' blocks alone 2.9).
 template <int Q_TOKENS>
 __global__ void __launch_bounds__(256)
 rope_kv4_write_kernel(const elem_t* qkv, long qkv_stride, elem_t* q_out, long q_stride, const float* __restrict__ table,
@@ -256,14 +261,14 @@ extern "C" int axk_rope_kv4_write(const void* qkv, long qkv_stride, void* q_out,
   AXK_REQUIRE((uintptr_t)table % 16 == 0, "rope_kv4_write: the table must be 16-byte aligned");
   if (n_tokens == 0) return 0;
   // Few tokens: a block each for its queries and for its keys and values.  Of 28 query and 4 key/value heads of 128 dims, so or in blocks of four
-  // and eight tokens: 8 single tokens 5.2 and 10.6 us, 128 8.7 and 13.7, 256 12.0 and 17.3; a portion of 64 tokens 7.8 and 10.0, of 256
-  // 8.4 and 10.3, of 512 9.6 and 10.6.  (Blocks of sixteen tokens take 33 us for 8192, of eight 31.)
-  const bool few = n_tokens <= 512;
-  const int rows = few ? 1 : 8, q_blocks = few ? n_tokens : ceil_div(n_tokens, 4), kv_blocks = write_kv ? ceil_div(n_tokens, rows) : 0;
+  // and eight tokens: 8 single tokens 4.7 and 9.4 us, 128 7.7 and 12.9, 512 17.9 and 21.1; a portion of 64 tokens 7.2 and 9.1, of 1024 9.6 and
+  // 10.9, of 2048 16.6 and 13.2.  Blocks of sixteen tokens: 1024 13.4, 4096 17.4 against 17.1 by eight, 8192 24.8 against 26.7.
+  const bool few = n_tokens <= 1024;
+  const int rows = few ? 1 : n_tokens <= 4096 ? 8 : LIST_ROWS, q_blocks = few ? n_tokens : ceil_div(n_tokens, 4), kv_blocks = write_kv ? ceil_div(n_tokens, rows) : 0;
   const unsigned blocks = q_blocks + kv_blocks;
 #define LAUNCH(Q_TOKENS)                                                                                                          \
   rope_kv4_write_kernel<Q_TOKENS><<<blocks, 256, 0, (hipStream_t)stream>>>(                                                       \
-      (const elem_t*)qkv, qkv_stride, (elem_t*)q_out, q_stride, table, positions, seq_rows, block_table, table_stride,            \
+      (const elem_t*)qkv, qkv_stride, (elem_t*)q_out, q_stride, rotary_dim > 0 ? table : (const float*)qkv, positions, seq_rows, block_table, table_stride,            \
       (unsigned char*)k_cache, (unsigned char*)v_cache, n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, page_size, kv_blocks, rows)
   if (few) LAUNCH(1);
   else LAUNCH(4);
