@@ -3,9 +3,14 @@
 //
 // Queries go there as half precision too, scaled by a power of two that brings a row's largest to 2^14 .. 2^15 (the score's
 // factor takes it back): bfloat16's eight bits fit with room, float32's 24 are three terms, each the rounding of what the ones before
-// it left, and three products.  The softmax's weights 2^(s - m + 14) are rounded to half precision, eleven bits (bfloat16
-// build; 2^-12 of a weight, an eighth of what the output's rounding takes), or are three such terms (float32 build).
-// Scores, maxima, sums and outputs are 32 bits.
+// it left, and three products.  The softmax's weights 2^(s - ref + 7), ref the column's largest score or up to 8 below it, are rounded to half
+// precision, eleven bits (bfloat16 build: 2^-11 of a weight, an eighth of the output's own 2^-8), or are three such terms
+// (float32 build).  Scores, maxima, sums and outputs are 32 bits.
+//
+// What they measure on an MI355X, of 28 query and 4 key heads of 128 dims in bfloat16 (a copy reaches 5.0 TB/s there, a product of 8,192^3 1.23
+// PFLOP/s): 8 tokens at 131,072 positions 124 us + 8 for the join, 605 MB at 4.9 TB/s; 8 at 32,768 36 + 5, 151 MB; one at 2,100 5.8 + 3.3, by waits
+// (a launch that does nothing takes 2.9, and each dependent trip to memory half a microsecond).  A prompt of 8,192 tokens 590 to 670 us with the
+// clock that the card's power allows, 0.72 to 0.82 PFLOP/s; one of 2,048 68 us; 512 tokens behind 1,536 59.
 #include <math.h>
 
 #include "api.h"
@@ -295,6 +300,8 @@ __device__ __forceinline__ float kv4_operands(Kv4Queries<HD>& q, float scale, u3
 // A workgroup has a chunk of a token and a set of up to sixteen query heads of a key head: grid (key heads x sets, work items).  Each of its
 // waves takes every KV4_WAVES-th block; what they sum is joined through LDS, in the order of the waves.  Of a token of one chunk the output
 // is stored at once; else output, reference and sum go to `partial` ([slot][head][chunk][HD], then [slot][head][chunk][2]).
+// Bound by the cache's bytes where there is work for the chip (three workgroups of 12 waves a CU have 110 KB of it on their way), by dependent trips
+// to memory where there is not.
 template <int HD>
 __global__ void __launch_bounds__(64 * KV4_WAVES, TERMS == 1 ? 3 : 2)
 kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned char* __restrict__ k_cache,
@@ -409,7 +416,8 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
 }
 
 // A token's chunks joined: with M the largest of their maxima, out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M); JOIN_SUMS sums side
-// by side over every JOIN_SUMS-th chunk, ascending, added in order.  grid (tokens, heads); a thread has four dims of one of the sums.
+// by side over every JOIN_SUMS-th chunk, ascending, added in order.  grid (tokens, heads); a thread has four dims of one of the sums.  Bound by its
+// launch: 3.3 us for one token of 9 chunks, 4.0 for 64, 7.6 for 8 of 128 chunks.
 #define JOIN_SUMS 8
 template <int HD>
 __global__ void __launch_bounds__(JOIN_SUMS * HD / 4)
@@ -482,6 +490,8 @@ kv4_join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ p
 // (four and a half bits a number, so few), beside the products of block b.
 // S^T = K Q^T and O^T = V^T P^T by 32x32x16 products: what a lane holds of the first is its operand of the second.  Row r of a tile
 // of S^T is position pi(r) of it, pi swapping bits 2 and 3, so that register e of tile pt is position 32 pt + 16 (e / 8) + 8 half + e % 8.
+// Of a block a wave has 32 products (1,024 cycles of its matrix core) and some 300 vector instructions, 33 of them exponentials; both run
+// beside each other, and with all CUs at work the card's power is what bounds them.  A tile alone takes 1.5 us a block.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 #define KV4_ROWS 128               // tokens of a tile
 // Positions lie in segments, 0 .. 2,047, .. 8,191, then 8,192 each.  What a row sums is closed at a segment's end and folded, in order, into what
@@ -919,7 +929,8 @@ kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned ch
                             partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);
 }
 
-// The segments of the tiles whose segments had a workgroup each, folded in order: rows (first token, count, -1 - segments, first slot).
+// The segments of the tiles whose segments had a workgroup each, folded in order: rows (first token, count, -1 - segments, first slot).  Bound by the
+// states' bytes (64 KB a segment of a head, 8 us for three tiles of two) or by its launch (4 us where no tile was cut).
 template <int HD>
 __global__ void __launch_bounds__(256)
 kv4_fold_kernel(elem_t* __restrict__ out, const int32_t* __restrict__ tiles, const float* __restrict__ partial, int n_slots, int n_heads) {
