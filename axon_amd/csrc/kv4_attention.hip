@@ -610,9 +610,10 @@ __device__ __forceinline__ void kv4_store(const Kv4State<HD>& st, float* at, int
   *reinterpret_cast<float2*>(at + KV4_ROWS * HD + (wave * 64 + lane) * 2) = make_float2(st.ref, st.l);
 }
 
-// Two states in order, one in the lanes (LATER: the second), one in memory, into the lanes.
-template <int HD, bool LATER>
-__device__ __forceinline__ void kv4_fold(Kv4State<HD>& st, const float* at, int wave, int lane) {
+// Two states in order, one in the lanes (LATER: the second), one in memory, into the lanes: of a tile of heads of HD dims, the groups of 32 dims
+// from dt0 on that the lanes have.
+template <int HD, bool LATER, int DIMS>
+__device__ __forceinline__ void kv4_fold(Kv4State<DIMS>& st, const float* at, int wave, int lane, int dt0) {
   const float2 other = *reinterpret_cast<const float2*>(at + KV4_ROWS * HD + (wave * 64 + lane) * 2);
   const float top = fmaxf(other.x, st.ref), base = top == -INFINITY ? 0.0f : top;
   const float f_other = __builtin_amdgcn_exp2f(__fsub_rn(other.x, base)), f_mine = __builtin_amdgcn_exp2f(__fsub_rn(st.ref, base));
@@ -620,10 +621,10 @@ __device__ __forceinline__ void kv4_fold(Kv4State<HD>& st, const float* at, int 
     return LATER ? __builtin_fmaf(theirs, f_other, __fmul_rn(mine, f_mine)) : __builtin_fmaf(mine, f_mine, __fmul_rn(theirs, f_other));
   };
 #pragma unroll
-  for (int dt = 0; dt < HD / 32; ++dt)
+  for (int dt = 0; dt < DIMS / 32; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float4 v = *reinterpret_cast<const float4*>(at + (((wave * (HD / 32) + dt) * 4 + g) * 64 + lane) * 4);
+      const float4 v = *reinterpret_cast<const float4*>(at + (((wave * (HD / 32) + dt0 + dt) * 4 + g) * 64 + lane) * 4);
       st.o[dt][4 * g] = join(st.o[dt][4 * g], v.x);
       st.o[dt][4 * g + 1] = join(st.o[dt][4 * g + 1], v.y);
       st.o[dt][4 * g + 2] = join(st.o[dt][4 * g + 2], v.z);
@@ -902,7 +903,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   }
   for (; b < seg_end; ++b) pass(b);
   if (!live || (segment < 0 && seg_first == seg_last)) continue;
-  if (kept) kv4_fold<HD, true>(st, state_at, wave & 3, lane);
+  if (kept) kv4_fold<HD, true>(st, state_at, wave & 3, lane, 0);
   if (seg_end < n_blocks || segment >= 0) {
     kv4_store<HD>(st, state_at, wave & 3, lane, nan_groups);
     nan_groups = 0;
@@ -929,31 +930,35 @@ kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned ch
                             partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);
 }
 
-// The segments of the tiles whose segments had a workgroup each, folded in order: rows (first token, count, -1 - segments, first slot).  Bound by the
-// states' bytes (64 KB a segment of a head, 8 us for three tiles of two) or by its launch (4 us where no tile was cut).
+// The segments of the tiles whose segments had a workgroup each, folded in order: rows (first token, count, -1 - segments, first slot).  grid (heads,
+// groups of 32 dims, KV4_FOLDS that share the rows); a thread has sixteen dims of a row of the tile, half of the group, as kv4_store left them.
+#define KV4_FOLDS 8
 template <int HD>
 __global__ void __launch_bounds__(256)
-kv4_fold_kernel(elem_t* __restrict__ out, const int32_t* __restrict__ tiles, const float* __restrict__ partial, int n_slots, int n_heads) {
-  const int32_t* mine = tiles + 4 * blockIdx.y;
-  const int t0 = mine[0], count = mine[1], segments = -1 - mine[2], slot = mine[3];
-  if (count <= 0 || count > KV4_ROWS || segments < 1 || slot < 0 || slot > n_slots - segments) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x, my_row = wave * 32 + (lane & 31);
-  if (wave * 32 >= count) return;
+kv4_fold_kernel(elem_t* __restrict__ out, const int32_t* __restrict__ tiles, int n_tiles, const float* __restrict__ partial, int n_slots, int n_heads) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x, dt = blockIdx.y, my_row = wave * 32 + (lane & 31);
   const size_t tile = (size_t)n_heads * Kv4State<HD>::FLOATS;
-  const float* at = partial + slot * tile + (size_t)head * Kv4State<HD>::FLOATS;
-  Kv4State<HD> st;
+  for (int first = 0, seen = 0; first < n_tiles; first += 64) {
+    uint64_t folds = __ballot(first + lane < n_tiles && tiles[4 * (first + lane) + 2] < -1);
+    for (; folds != 0; folds &= folds - 1) {
+      if (seen++ % KV4_FOLDS != (int)blockIdx.z) continue;
+      const int32_t* mine = tiles + 4 * (first + __builtin_ctzll(folds));
+      const int t0 = mine[0], count = mine[1], segments = -1 - mine[2], slot = mine[3];
+      if (count <= 0 || count > KV4_ROWS || slot < 0 || slot > n_slots - segments || wave * 32 >= count) continue;
+      const float* at = partial + slot * tile + (size_t)head * Kv4State<HD>::FLOATS;
+      Kv4State<32> st;
 #pragma unroll
-  for (int dt = 0; dt < HD / 32; ++dt)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float4 v = *reinterpret_cast<const float4*>(at + (((wave * (HD / 32) + dt) * 4 + g) * 64 + lane) * 4);
-      st.o[dt][4 * g] = v.x; st.o[dt][4 * g + 1] = v.y; st.o[dt][4 * g + 2] = v.z; st.o[dt][4 * g + 3] = v.w;
+      for (int g = 0; g < 4; ++g) {
+        const float4 v = *reinterpret_cast<const float4*>(at + (((wave * (HD / 32) + dt) * 4 + g) * 64 + lane) * 4);
+        st.o[0][4 * g] = v.x; st.o[0][4 * g + 1] = v.y; st.o[0][4 * g + 2] = v.z; st.o[0][4 * g + 3] = v.w;
+      }
+      const float2 own = *reinterpret_cast<const float2*>(at + KV4_ROWS * HD + (wave * 64 + lane) * 2);
+      st.ref = own.x;
+      st.l = own.y;
+      for (int s = 1; s < segments; ++s) kv4_fold<HD, false>(st, at + s * tile, wave, lane, dt);
+      if (my_row < count) kv4_store_row<32>(st, out + ((size_t)(t0 + my_row) * n_heads + head) * HD + dt * 32, lane, 0);
     }
-  const float2 own = *reinterpret_cast<const float2*>(at + KV4_ROWS * HD + (wave * 64 + lane) * 2);
-  st.ref = own.x;
-  st.l = own.y;
-  for (int s = 1; s < segments; ++s) kv4_fold<HD, false>(st, at + s * tile, wave, lane);
-  if (my_row < count) kv4_store_row<HD>(st, out + ((size_t)(t0 + my_row) * n_heads + head) * HD, lane, 0);
+  }
 }
 
 // ============================================================================ entry points
@@ -1068,10 +1073,9 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
 #undef LAUNCH
   AXK_LAUNCH_CHECK("kv4_attention_prefill");
   if (n_slots > 0) {
-    if (head_dim == 64)
-      kv4_fold_kernel<64><<<dim3(n_heads, n_tiles), 256, 0, (hipStream_t)stream>>>((elem_t*)out, tiles, partial, n_slots, n_heads);
-    else
-      kv4_fold_kernel<128><<<dim3(n_heads, n_tiles), 256, 0, (hipStream_t)stream>>>((elem_t*)out, tiles, partial, n_slots, n_heads);
+    const dim3 folds(n_heads, head_dim / 32, KV4_FOLDS);
+    if (head_dim == 64) kv4_fold_kernel<64><<<folds, 256, 0, (hipStream_t)stream>>>((elem_t*)out, tiles, n_tiles, partial, n_slots, n_heads);
+    else kv4_fold_kernel<128><<<folds, 256, 0, (hipStream_t)stream>>>((elem_t*)out, tiles, n_tiles, partial, n_slots, n_heads);
     AXK_LAUNCH_CHECK("kv4_attention_prefill");
   }
   return 0;
