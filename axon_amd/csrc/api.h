@@ -538,8 +538,10 @@ int axk_kv4_attention_decode(const void* q, int q_stride, const void* k_cache, c
                              void* stream);
 // Prompt portions: tiles [n_tiles][4] = (first token, count up to axk_kv4_prefill_tile, segment, slot).  segment -1: everything that the
 // tile's rows see, which needs a slot of the workspace (its own, else -1) if that lies in several segments of positions
-// (axk_kv4_prefill_segment); segment s: only the positions from axk_kv4_prefill_segment_start(s) up to the next, into its slot; segment -1 - n: the tile's n segments, which lie in
-// n slots from `slot` on, are folded into its rows of out (by a second launch).  The same bits either way.
+// (axk_kv4_prefill_segment); segment s: only the positions from axk_kv4_prefill_segment_start(s) up to the next, into its slot.  A tile that is
+// cut has a row for each of its n segments, their slots in order, of which the first says n << axk_kv4_prefill_many() | s: a second
+// launch folds them into the tile's rows of out.  The same bits either way.
+int axk_kv4_prefill_many(void);
 int axk_kv4_prefill_tile(void);
 int axk_kv4_prefill_segment(int position);
 int axk_kv4_prefill_segment_start(int segment);

@@ -494,13 +494,15 @@ kv4_join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ p
 // beside each other, and with all CUs at work the card's power is what bounds them.  A tile alone takes 1.5 us a block.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 #define KV4_ROWS 128               // tokens of a tile
-// Positions lie in segments, 0 .. 2,047, .. 8,191, then 8,192 each.  What a row sums is closed at a segment's end and folded, in order, into what
-// the segments before gave, whether one workgroup takes them all (its sums then wait in the workspace) or one each, which
+// Positions lie in segments that end at 1,024, 2,048, 4,096, 8,192 and every 8,192 behind.  What a row sums is closed at a segment's end and folded,
+// in order, into what the segments before gave, whether one workgroup takes them all (its sums then wait in the workspace) or one each, which
 // kv4_fold_kernel joins: the same bits, so a row's result does not depend on how many tiles a step has.  Workgroups that began together
-// get to a segment's end together, and their 128 KB each take 6 us there and 6 back: a prompt of 8,192 tokens 649 us without segments, 700
-// with segments of 2,048 throughout, 667 so; 980 tokens in ragged portions up to 4,400 positions 130 us without, 89 so.
-__host__ __device__ inline int kv4_segment_of(int p) { return p < 2048 ? 0 : p < 8192 ? 1 : 1 + p / 8192; }
-__host__ __device__ inline int kv4_segment_start(int s) { return s < 2 ? s * 2048 : s > 262144 ? 0x7fffffff : (s - 1) * 8192; }
+// get to a segment's end together, and their 128 KB each take 6 us there and 6 back.  With ends at 2,048 and 8,192 alone / these, 28 heads over 4 of 128 dims:
+// 512 tokens behind 1,536 60 / 39 + 6 us, 980 in ragged portions up to 4,400 positions 81 + 5 / 68 + 9, a prompt of 2,048 69 / 63 + 9, of 4,096 179 /
+// 190, of 8,192 670 / 685 (without ends 650; with one every 2,048 700).
+#define KV4_MANY 20                // a cut tile's first row names its segment and, from this bit on, how many there are
+__host__ __device__ inline int kv4_segment_of(int p) { return p < 1024 ? 0 : p < 2048 ? 1 : p < 4096 ? 2 : p < 8192 ? 3 : 3 + p / 8192; }
+__host__ __device__ inline int kv4_segment_start(int s) { return s < 3 ? s * 1024 : s == 3 ? 4096 : s > 262146 ? 0x7fffffff : (s - 3) * 8192; }
 
 __device__ __forceinline__ f32x16 kv4_mma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -914,7 +916,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   kv4_store_row<HD>(st, out_row, lane, nan_groups);
 }
 
-// tiles [n][4] = (first token, count, segment or -1 for all that the tile sees, slot of the workspace); a segment below -1 is kv4_fold_kernel's.
+// tiles [n][4] = (first token, count, segment or -1 for all that the tile sees, slot of the workspace).
 template <int HD, int HPB>
 __global__ void __launch_bounds__(256 * HPB, TERMS == 1 ? 2 : 1)
 kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned char* __restrict__ k_cache,
@@ -924,14 +926,16 @@ kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned ch
                    int window, float scale) {
   extern __shared__ __align__(256) unsigned char smem[];
   const int32_t* mine = tiles + 4 * blockIdx.y;
-  const int t0 = mine[0], count = mine[1], segment = mine[2], slot = mine[3];
+  const int t0 = mine[0], count = mine[1], segment = mine[2] < 0 ? mine[2] : mine[2] & ((1 << KV4_MANY) - 1), slot = mine[3];
   if (count <= 0 || count > KV4_ROWS || segment < -1) return;
   kv4_prefill_tile<HD, HPB>(smem, t0, count, q, q_stride, k_cache, v_cache, block_table, table_stride, positions, seq_rows, out, segment, slot,
                             partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);
 }
 
-// The segments of the tiles whose segments had a workgroup each, folded in order: rows (first token, count, -1 - segments, first slot).  grid (heads,
-// groups of 32 dims, KV4_FOLDS that share the rows); a thread has sixteen dims of a row of the tile, half of the group, as kv4_store left them.
+// The segments of the tiles whose segments had a workgroup each, folded in order: rows that say how many there are, which lie in as many slots from
+// theirs on.  grid (heads, groups of 32 dims, KV4_FOLDS that share the rows); a thread has sixteen dims of a row of the tile, half of the group, as
+// kv4_store left them.  Bound by its launch (2.9 us of one that does nothing) and two trips to memory: 5.6 us for four tiles of two segments
+// of 28 heads of 128 dims, 13 for eight of up to four, 4.7 where nothing was cut.
 #define KV4_FOLDS 8
 template <int HD>
 __global__ void __launch_bounds__(256)
@@ -939,11 +943,11 @@ kv4_fold_kernel(elem_t* __restrict__ out, const int32_t* __restrict__ tiles, int
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x, dt = blockIdx.y, my_row = wave * 32 + (lane & 31);
   const size_t tile = (size_t)n_heads * Kv4State<HD>::FLOATS;
   for (int first = 0, seen = 0; first < n_tiles; first += 64) {
-    uint64_t folds = __ballot(first + lane < n_tiles && tiles[4 * (first + lane) + 2] < -1);
+    uint64_t folds = __ballot(first + lane < n_tiles && tiles[4 * (first + lane) + 2] >> KV4_MANY > 0);
     for (; folds != 0; folds &= folds - 1) {
       if (seen++ % KV4_FOLDS != (int)blockIdx.z) continue;
       const int32_t* mine = tiles + 4 * (first + __builtin_ctzll(folds));
-      const int t0 = mine[0], count = mine[1], segments = -1 - mine[2], slot = mine[3];
+      const int t0 = mine[0], count = mine[1], segments = mine[2] >> KV4_MANY, slot = mine[3];
       if (count <= 0 || count > KV4_ROWS || slot < 0 || slot > n_slots - segments || wave * 32 >= count) continue;
       const float* at = partial + slot * tile + (size_t)head * Kv4State<HD>::FLOATS;
       Kv4State<32> st;
@@ -1020,6 +1024,7 @@ extern "C" int axk_kv4_attention_decode(const void* q, int q_stride, const void*
   return 0;
 }
 
+extern "C" int axk_kv4_prefill_many(void) { return KV4_MANY; }
 extern "C" int axk_kv4_prefill_segment(int position) { return kv4_segment_of(position); }
 extern "C" int axk_kv4_prefill_segment_start(int segment) { return kv4_segment_start(segment); }
 
@@ -1062,8 +1067,9 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
         positions, seq_rows, (elem_t*)out, tiles, partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);             \
   }
 #if AXON_BF16
-  // one query head a workgroup while two such workgroups a CU are enough; beyond that two, which share what is unpacked
-  if (group >= 2 && (long)n_tiles * n_heads > 512) {
+  // One query head a workgroup while there are up to three a CU, which spread better; beyond that two, which share what is unpacked: 672 tiles and
+  // heads in ragged portions 68 against 73 us, 616 of a prompt of 2,800 tokens 103 against 110, 896 of one of 4,096 199 against 190.
+  if (group >= 2 && (long)n_tiles * n_heads > 768) {
     if (head_dim == 64) LAUNCH(64, 2) else LAUNCH(128, 2)
   } else
 #endif

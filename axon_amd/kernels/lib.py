@@ -192,7 +192,7 @@ _SIGNATURES = {
 _PLAIN = ["axk_argmax_workspace", "axk_attention_decode_chunk", "axk_attention_decode_item_factor", "axk_attention_decode_workspace",
           "axk_attention_prefill_tile", "axk_delta_chunked_workspace", "axk_gemm_workspace", "axk_latent_attention_workspace",
           "axk_masked_attention_workspace", "axk_packed_elems", "axk_kv4_decode_chunk", "axk_kv4_decode_item_factor",
-          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile", "axk_kv4_prefill_segment",
+          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile", "axk_kv4_prefill_many", "axk_kv4_prefill_segment",
           "axk_kv4_prefill_segment_start", "axk_kv4_prefill_workspace"]
 
 
@@ -1842,9 +1842,9 @@ class Kernels:
     def kv4_prefill_tiles(self, spans, window: int, n_heads: int, n_kv_heads: int) -> List[tuple]:
         """The tiles of `kv4_attention_prefill` for portions (first token of the step, tokens, position of the first): rows of (first
         token, count, segment, slot of the workspace), those with the most work first.  A tile whose rows see several segments of positions is
-        cut there where a step has few tiles (its segments then run side by side, and a last row has them folded); the bits are
-        the same either way."""
-        tile = int(self.run.axk_kv4_prefill_tile())
+        cut there where a step has few tiles (its segments then run side by side, and are folded behind them; the first one's row
+        has their number above the segment's); the bits are the same either way."""
+        tile, many = int(self.run.axk_kv4_prefill_tile()), int(self.run.axk_kv4_prefill_many())
         segment_of, start_of = self.run.axk_kv4_prefill_segment, self.run.axk_kv4_prefill_segment_start
         runs = []
         for start, length, at in spans:
@@ -1856,26 +1856,24 @@ class Kernels:
         # two workgroups of one head fit a CU: fewer than that, and tiles are cut (a tile at 30,000 positions alone takes 28 of 256 CUs
         # 0.8 ms, and cut 0.2)
         cut = len(runs) * n_heads < 512
-        rows, folds, slots = [], [], 0
+        rows, slots = [], 0
         for start, n, low, high in runs:
             first, last = int(segment_of(low)), int(segment_of(high))
             if first == last:
                 rows.append((high - low, start, n, -1, -1))
-            elif not cut:
+            elif not cut or last - first >= 1 << 31 - many - 1:
                 rows.append((high - low, start, n, -1, slots))
                 slots += 1
             else:
-                rows += [(min(high, int(start_of(s + 1)) - 1) - max(low, int(start_of(s))), start, n, s, slots + s - first)
-                         for s in range(first, last + 1)]
-                folds.append((start, n, -1 - (last - first + 1), slots))
+                rows += [(min(high, int(start_of(s + 1)) - 1) - max(low, int(start_of(s))), start, n,
+                          s | (last - first + 1 << many if s == first else 0), slots + s - first) for s in range(first, last + 1)]
                 slots += last - first + 1
         rows.sort(key=lambda r: -r[0])
-        return [r[1:] for r in rows] + folds
+        return [r[1:] for r in rows]
 
     def kv4_prefill_workspace(self, tiles, n_heads: int, head_dim: int) -> int:
         """Floats of `kv4_attention_prefill`'s workspace for these tiles (as `kv4_prefill_tiles` lists them)."""
-        slots = max((row[3] + (-1 - row[2] if row[2] < -1 else 1) for row in tiles), default=0)
-        return int(self.run.axk_kv4_prefill_workspace(slots, n_heads, head_dim))
+        return int(self.run.axk_kv4_prefill_workspace(max((row[3] + 1 for row in tiles), default=0), n_heads, head_dim))
 
     def kv4_attention_prefill(self, q, q_stride, k_cache, v_cache, block_table, positions, seq_rows, out, tiles, partial, n_heads,
                               n_kv_heads, head_dim, page_size, window, scale) -> torch.Tensor:

@@ -28,7 +28,7 @@ def test_tiles_have_every_row_and_position_once(seed, nh, nkv, window):
     tiles = k.kv4_prefill_tiles(spans, window, nh, nkv)
     start, segment = k.run.axk_kv4_prefill_segment_start, k.run.axk_kv4_prefill_segment
     at_of = {s + i: at + i for s, n, at in spans for i in range(n)}
-    rows, slots, parts, work = [], set(), {}, []
+    rows, slots, parts, work, many = [], set(), {}, [], int(k.run.axk_kv4_prefill_many())
     for first, count, which, slot in tiles:
         assert 0 < count <= TILE
         p0, p1 = at_of[first], at_of[first + count - 1]
@@ -36,20 +36,22 @@ def test_tiles_have_every_row_and_position_once(seed, nh, nkv, window):
         low = max(0, p0 + 1 - window) if window else 0
         s0, s1 = segment(low), segment(p1)
         if which >= 0:
-            assert s0 <= which <= s1 and slot not in slots
+            n, which = which >> many, which & ((1 << many) - 1)
+            assert s0 <= which <= s1 and slot not in slots and n == (s1 - s0 + 1 if which == s0 else 0)
             slots.add(slot)
             parts.setdefault((first, count), {})[which] = slot
             work.append(min(p1, start(which + 1) - 1) - max(low, start(which)))
-        elif which == -1:
+        else:
+            assert which == -1 and (slot == -1) == (s0 == s1) and slot not in slots
             rows += range(first, first + count)
-            assert (slot == -1) == (s0 == s1) and slot not in slots
             slots |= {slot} - {-1}
             work.append(p1 - low)
-        else:                                             # a fold: its segments' slots, in order
-            mine = parts.pop((first, count))
-            assert -1 - which == s1 - s0 + 1 and [mine[s] for s in range(s0, s1 + 1)] == list(range(slot, slot + s1 - s0 + 1))
-            rows += range(first, first + count)
-    assert not parts and sorted(rows) == sorted(at_of) and work == sorted(work, reverse=True)
+    for (first, count), mine in parts.items():              # the slots of a tile's segments, in order
+        p1 = at_of[first + count - 1]
+        low = max(0, p1 - count + 2 - window) if window else 0
+        assert [mine[s] for s in range(segment(low), segment(p1) + 1)] == list(range(mine[segment(low)], mine[segment(low)] + len(mine)))
+        rows += range(first, first + count)
+    assert sorted(rows) == sorted(at_of) and work == sorted(work, reverse=True)
     assert slots == set(range(len(slots)))
     one = k.kv4_prefill_workspace([(0, 1, -1, 0)], nh, 64)
     assert one > 0 and k.kv4_prefill_workspace(tiles, nh, 64) == len(slots) * one
@@ -59,9 +61,9 @@ def test_segments_follow_each_other():
     k = kernels("bfloat16")
     segment, start = k.run.axk_kv4_prefill_segment, k.run.axk_kv4_prefill_segment_start
     for s in range(300):
-        assert start(s) < start(s + 1) and start(s) % 64 == 0
+        assert start(s) < start(s + 1) and start(s) % 64 == 0 and s < 1 << int(k.run.axk_kv4_prefill_many())
         assert segment(start(s)) == s == segment(start(s + 1) - 1)
-    assert segment(2 ** 31 - 1) > 0 and start(segment(2 ** 31 - 1) + 1) == 2 ** 31 - 1
+    assert 0 < segment(2 ** 31 - 1) < 1 << int(k.run.axk_kv4_prefill_many()) and start(segment(2 ** 31 - 1) + 1) == 2 ** 31 - 1
 
 
 @pytest.mark.parametrize("window", [0, 1, 300, 9000])
