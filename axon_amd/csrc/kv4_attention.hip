@@ -10,7 +10,7 @@
 // What they measure on an MI355X, of 28 query and 4 key heads of 128 dims in bfloat16 (a copy reaches 5.0 TB/s there, a product of 8,192^3 1.23
 // PFLOP/s): 8 tokens at 131,072 positions 124 us + 8 for the join, 605 MB at 4.9 TB/s; 8 at 32,768 36 + 5, 151 MB; one at 2,100 5.8 + 3.3, by waits
 // (a launch that does nothing takes 2.9, and each dependent trip to memory half a microsecond).  A prompt of 8,192 tokens 590 to 670 us with the
-// clock that the card's power allows, 0.72 to 0.82 PFLOP/s; one of 2,048 68 us; 512 tokens behind 1,536 59.
+// clock that the card's power allows, 0.72 to 0.82 PFLOP/s; one of 2,048 63 + 9; 512 tokens behind 1,536 39 + 6.
 #include <math.h>
 
 #include "api.h"
@@ -490,8 +490,9 @@ kv4_join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ p
 // (four and a half bits a number, so few), beside the products of block b.
 // S^T = K Q^T and O^T = V^T P^T by 32x32x16 products: what a lane holds of the first is its operand of the second.  Row r of a tile
 // of S^T is position pi(r) of it, pi swapping bits 2 and 3, so that register e of tile pt is position 32 pt + 16 (e / 8) + 8 half + e % 8.
-// Of a block a wave has 32 products (1,024 cycles of its matrix core) and some 300 vector instructions, 33 of them exponentials; both run
-// beside each other, and with all CUs at work the card's power is what bounds them.  A tile alone takes 1.5 us a block.
+// Of a block a wave has 32 products (1,024 cycles of its matrix core), 235 vector instructions, 32 of them exponentials, and 32 KB of LDS to read: of a prompt
+// of 8,192 tokens the matrix cores are at work for 42 % of the cycles, the vector units for 57 %, LDS for some 55 %, at the 1.8 GHz that
+// the card's power allows then.  A tile alone takes 1.5 us a block.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 #define KV4_ROWS 128               // tokens of a tile
 // Positions lie in segments that end at 1,024, 2,048, 4,096, 8,192 and every 8,192 behind.  What a row sums is closed at a segment's end and folded,
@@ -510,7 +511,9 @@ __device__ __forceinline__ f32x16 kv4_mma32(u32x4 a, u32x4 b, f32x16 c) {
 
 template <int HD>
 struct Kv4Stage {
-  static constexpr int K_BYTES = KV4_BLOCK * HD * 2, BYTES = 2 * K_BYTES, ALL = 2 * BYTES + 2 * (HD / 4);
+  static constexpr int BYTES = KV4_BLOCK * HD * 2, NANS = HD / 4;     // of a block's keys or values, of its values that are not numbers
+  // two blocks' keys, V blocks' values and what is not a number among them
+  static constexpr int all(int v) { return 2 * BYTES + v * (BYTES + NANS); }
   // a row's pieces are permuted by this
   __device__ static __forceinline__ int k_swizzle(int row) { return HD == 128 ? row & 15 : (row >> 1) & 7; }
   __device__ static __forceinline__ int v_swizzle(int dim) { return (dim >> 1) & 7; }
@@ -518,7 +521,7 @@ struct Kv4Stage {
   __device__ static __forceinline__ int k_at(int row, int chunk) {
     return row * (HD * 2) + ((chunk ^ k_swizzle(row)) << 4);
   }
-  __device__ static __forceinline__ int v_at(int dim, int octet) { return K_BYTES + dim * 128 + ((octet ^ v_swizzle(dim)) << 4); }
+  __device__ static __forceinline__ int v_at(int dim, int octet) { return dim * 128 + ((octet ^ v_swizzle(dim)) << 4); }
 };
 
 // An octet of slots of one head on its way: a lane has HD/64 words of a row of K (eight lanes a row) and of V^T (neighbouring dims).
@@ -564,10 +567,10 @@ __device__ __forceinline__ void kv4_edge(Kv4Octet<HD>& in, int octet, int p, int
   in.v_scale = make_uint4(metas[0], metas[1], metas[2], metas[3]);
 }
 
-// Unpacked into a stage, as octet `octet` of its block, in PIECES pieces (0, 1: keys, 2, 3: values).
+// Unpacked into its stages, as octet `octet` of its block, in PIECES pieces (0, 1: keys, 2, 3: values).
 #define KV4_PIECES 4
 template <int HD>
-__device__ __forceinline__ void kv4_unpack(const Kv4Octet<HD>& in, unsigned char* stage, int octet, int piece, const Kv4Masks& masks, int lane) {
+__device__ __forceinline__ void kv4_unpack(const Kv4Octet<HD>& in, unsigned char* k_stage, unsigned char* v_stage, int octet, int piece, const Kv4Masks& masks, int lane) {
   half2_t sc[4], cc[4];
   const int w = piece & 1;
   if (w >= HD / 64) return;
@@ -575,13 +578,13 @@ __device__ __forceinline__ void kv4_unpack(const Kv4Octet<HD>& in, unsigned char
     kv4_pair_scale(in.k_scale | in.k_scale << 16, sc[0], cc[0]);
 #pragma unroll
     for (int i = 1; i < 4; ++i) { sc[i] = sc[0]; cc[i] = cc[0]; }
-    *reinterpret_cast<u32x4*>(stage + Kv4Stage<HD>::k_at(8 * octet + (lane >> 3), (lane & 7) * (HD / 64) + w)) =
+    *reinterpret_cast<u32x4*>(k_stage + Kv4Stage<HD>::k_at(8 * octet + (lane >> 3), (lane & 7) * (HD / 64) + w)) =
         kv4_operand(in.k[w], sc, cc, masks);
   } else {
     const unsigned metas[4] = {in.v_scale.x, in.v_scale.y, in.v_scale.z, in.v_scale.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) kv4_pair_scale(metas[i], sc[i], cc[i]);
-    *reinterpret_cast<u32x4*>(stage + Kv4Stage<HD>::v_at(lane * (HD / 64) + w, octet)) = kv4_operand(in.v[w], sc, cc, masks);
+    *reinterpret_cast<u32x4*>(v_stage + Kv4Stage<HD>::v_at(lane * (HD / 64) + w, octet)) = kv4_operand(in.v[w], sc, cc, masks);
   }
 }
 
@@ -665,7 +668,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
                                                  elem_t* __restrict__ out, int segment, int slot, float* __restrict__ partial, int n_slots,
                                                  int n_heads, int n_kv_heads, int page_size, int window, float scale) {
   using S = Kv4Stage<HD>;
-  constexpr int WAVES = 4 * HPB, OCTETS = 8 / WAVES, DT = HD / 32, KS = HD / 16;
+  constexpr int WAVES = 4 * HPB, OCTETS = 8 / WAVES, DT = HD / 32, KS = HD / 16, V_STAGES = 1 + HPB;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
   const int group = n_heads / n_kv_heads, sets = (group + HPB - 1) / HPB, kvh = blockIdx.x / sets;
   const int in_group = (blockIdx.x % sets) * HPB + (wave >> 2), head = kvh * group + min(in_group, group - 1);
@@ -695,7 +698,9 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   const size_t head_bytes = (size_t)page_size * kv4_row_bytes(HD), page_bytes = head_bytes * n_kv_heads, head_at = head_bytes * kvh;
   const int shift = __builtin_ctz(page_size);
   Kv4Masks masks = kv4_masks();
-  unsigned char* nans_of = smem + 2 * S::BYTES;
+  auto k_at = [](int b) { return (b & 1) * S::BYTES; };
+  auto v_at = [](int b) { return 2 * S::BYTES + (int)((unsigned)b % V_STAGES) * S::BYTES; };
+  auto nans_of = [&](int b) { return smem + (2 + V_STAGES) * S::BYTES + (unsigned)b % V_STAGES * S::NANS; };
   // an octet past the tile's last position: its page's
   auto place = [&](int b, int n) { return min(base + b * KV4_BLOCK + 8 * (n * WAVES + wave), last); };
   auto edge = [&](int b) { return base + b * KV4_BLOCK < tile_lo || base + b * KV4_BLOCK + KV4_BLOCK - 1 > pos0; };
@@ -713,11 +718,11 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     if (edge(b))
 #pragma unroll
       for (int n = 0; n < OCTETS; ++n)
-        kv4_edge<HD>(octets[n], n * WAVES + wave, base + b * KV4_BLOCK + 8 * (n * WAVES + wave), first, last, nans_of + (b & 1) * (HD / 4), lane);
+        kv4_edge<HD>(octets[n], n * WAVES + wave, base + b * KV4_BLOCK + 8 * (n * WAVES + wave), first, last, nans_of(b), lane);
   };
   auto unpack = [&](int b, int piece) {
 #pragma unroll
-    for (int n = 0; n < OCTETS; ++n) kv4_unpack<HD>(octets[n], smem + (b & 1) * S::BYTES, n * WAVES + wave, piece, masks, lane);
+    for (int n = 0; n < OCTETS; ++n) kv4_unpack<HD>(octets[n], smem + k_at(b), smem + v_at(b), n * WAVES + wave, piece, masks, lane);
   };
   auto unpack_all = [&](int b) {
 #pragma unroll
@@ -784,6 +789,10 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     kv4_meet();
   };
   const int from = live ? max(0, wave_first - base) / KV4_BLOCK : n_blocks, to = live ? min((wave_last - base) / KV4_BLOCK, n_blocks - 1) : -1;
+  // The second head's waves meet the others between a block's scores and its weights: the matrix cores have the products of the one head's scores
+  // while the vector unit has the weights of the other's block before.  (So its values are read while those two blocks on are unpacked.)  Prompts of
+  // 3,600 tokens 160 -> 155 us, of 6,000 412 -> 398; of 8,192, where the card's power bounds it, within 1 %.
+  const bool late = HPB == 2 && wave >= 4;
   unsigned nan_groups = 0;                         // groups of 32 dims in which the lane's row sees a value that is not a number
   bool kept = false;                               // segments before this one wait in the workspace
   for (int b = 0, seg_end; b < n_blocks; b = seg_end) {
@@ -796,8 +805,8 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     {
       // A row begins at a multiple of its size, and piece 2 n + half of it is piece `half` with n's bits exclusive-ored in: one instruction from a
       // base each.  The bases are opaque, or the compiler keeps every address in a register across the loop.
-      unsigned k_base = lds0 + (b & 1) * S::BYTES + k_row * (HD * 2) + ((half ^ S::k_swizzle(k_row)) << 4);
-      unsigned v_base = lds0 + (b & 1) * S::BYTES + S::K_BYTES + l32 * 128 + ((half ^ S::v_swizzle(l32)) << 4);
+      unsigned k_base = lds0 + k_at(b) + k_row * (HD * 2) + ((half ^ S::k_swizzle(k_row)) << 4);
+      unsigned v_base = lds0 + v_at(b) + l32 * 128 + ((half ^ S::v_swizzle(l32)) << 4);
       asm volatile("" : "+v"(k_base), "+v"(v_base));
       // The scores, fragments read two groups of products ahead, and the next block unpacked a piece behind each group: the matrix cores
       // work on the group meanwhile.
@@ -836,6 +845,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
       }
       ask(b + 2);
       look_up(b + 3);
+      if (late) kv4_meet();
       const bool whole = p0 + KV4_BLOCK - 1 <= wave_hi && p0 >= wave_lo;
       if (!whole) {
         int from = p0 + 8 * half;
@@ -898,10 +908,10 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
                        high = my_pos >= p0 + 63 ? ~0ull : ~(~0ull << max(my_pos - p0 + 1, 0));
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-          if (*reinterpret_cast<const uint64_t*>(nans_of + (b & 1) * (HD / 4) + 8 * dt) & low & high) nan_groups |= 1u << dt;
+          if (*reinterpret_cast<const uint64_t*>(nans_of(b) + 8 * dt) & low & high) nan_groups |= 1u << dt;
       }
     }
-    kv4_meet();
+    if (!late) kv4_meet();
   }
   for (; b < seg_end; ++b) pass(b);
   if (!live || (segment < 0 && seg_first == seg_last)) continue;
@@ -1050,7 +1060,7 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
   const int n_slots = (int)(slots < 1 << 30 ? slots : 1 << 30);
 #define LAUNCH(HD, HPB)                                                                                                         \
   {                                                                                                                             \
-    constexpr int lds = Kv4Stage<HD>::ALL;                                                                                      \
+    constexpr int lds = Kv4Stage<HD>::all(1 + HPB);                                                                                      \
     static uint64_t configured = 0;                                                            /* a bit for each device */      \
     int device = 0;                                                                                                             \
     hipError_t e = hipGetDevice(&device);                                                                                       \
