@@ -244,3 +244,43 @@ def test_refusals_of_write_and_read():
     none = dict(positions=i32([]).reshape(0), seq_rows=i32([]).reshape(0))
     k.kv4_read(**{**read, **none, "k_out": rows[0][:0], "v_out": rows[1][:0]})
     k.rope_kv4_write(**{**write, **none, "qkv": qkv[:0], "q_out": qkv[:0, :nh * dim], "table": torch.zeros((0, 16, 2), device="cuda")})
+
+
+@pytest.mark.parametrize("dim,nh,nkv,spans,window", [(128, 7, 1, [(300, 5), (130, 0), (77, 1000)], 0), (64, 4, 2, [(257, 700), (64, 64)], 130),
+                                                     (128, 3, 1, [(128, 1990), (200, 4000)], 2500)])
+def test_one_and_two_heads_a_workgroup_give_the_same_bits(dim, nh, nkv, spans, window):
+    """With windows, segments and groups that are not numbers in the middle, at the edges of what is seen and beyond: rows of nothing make the
+    step one of many tiles."""
+    k, page = kernels("bfloat16"), 32
+    held = Held([n + at for n, at in spans], nkv, dim, page, seed=80)
+    rng = np.random.default_rng(4)
+    for cache, keys in ((held.args[0], True), (held.args[1], False)):
+        scales = cache.view(-1, nkv, page * P.row_bytes(dim))[..., page * dim // 2:].view(torch.int16)
+        for r, (n, at) in enumerate(spans):
+            for p in rng.integers(0, n + at, 3):
+                row = scales[int(held.table[r, p // page])]
+                if keys and p > at + n // 2:                            # (late keys: else every row is NaN throughout)
+                    row.view(nkv, page, dim // 32)[0, p % page, 1] = 0x7FE0
+                elif not keys:
+                    row.view(nkv, page // 8, dim // 32, 8)[nkv - 1, p % page // 8, 0, p % 8] = 0x7FE0
+    T = sum(n for n, _ in spans)
+    pos = [at + i for n, at in spans for i in range(n)]
+    seq = [r for r, (n, _) in enumerate(spans) for _ in range(n)]
+    firsts = np.cumsum([0] + [n for n, _ in spans])[:-1]
+    q = torch.randn((T, nh * dim), generator=torch.Generator().manual_seed(9)).bfloat16().cuda()
+    cut = k.kv4_prefill_tiles([(int(f), n, at) for f, (n, at) in zip(firsts, spans)], window, nh, nkv)
+    whole = [(int(f) + i, min(128, n - i), -1, -1) for f, (n, _) in zip(firsts, spans) for i in range(0, n, 128)]
+    whole = [(a, b, c, i) for i, (a, b, c, _) in enumerate(whole)]
+    few = len(cut) * nh, len(whole) * nh
+    assert max(few) <= 768
+    nothing = [(0, 0, -1, -1)] * (769 // nh + 1)
+    want = None
+    for tiles in (cut, cut + nothing, whole, nothing + whole):
+        out = torch.full((T, nh * dim), 5.0, dtype=q.dtype, device="cuda")
+        partial = torch.full((k.kv4_prefill_workspace(tiles, nh, dim),), float("nan"), device="cuda")
+        k.kv4_attention_prefill(q, nh * dim, *held.args, i32(pos), i32(seq), out, i32(tiles), partial, nh, nkv, dim, page, window, 0.1)
+        want = out if want is None else want
+        assert torch.equal(out.view(torch.int16), want.view(torch.int16))
+    assert want.isnan().any() and want.isfinite().any() and not (want == 5.0).all(-1).any()
+    single = decode(k, held, q, pos, seq, nh, nkv, dim, page, window, 0.1)
+    assert torch.equal(single.isnan(), want.isnan())
