@@ -8,9 +8,9 @@
 // (float32 build).  Scores, maxima, sums and outputs are 32 bits.
 //
 // What they measure on an MI355X, of 28 query and 4 key heads of 128 dims in bfloat16 (a copy reaches 5.0 TB/s there, a product of 8,192^3 1.23
-// PFLOP/s): 8 tokens at 131,072 positions 124 us + 8 for the join, 605 MB at 4.9 TB/s; 8 at 32,768 36 + 5, 151 MB; one at 2,100 5.8 + 3.3, by waits
-// (a launch that does nothing takes 2.9, and each dependent trip to memory half a microsecond).  A prompt of 8,192 tokens 590 to 670 us with the
-// clock that the card's power allows, 0.72 to 0.82 PFLOP/s; one of 2,048 63 + 9; 512 tokens behind 1,536 39 + 6.
+// PFLOP/s): 8 tokens at 131,072 positions 124 us + 8 for the join, 605 MB at 4.9 TB/s; 8 at 32,768 36 + 5, 151 MB; one at 2,100 5.8 + 3.3,
+// by waits (a launch that does nothing takes 2.9, and each dependent trip to memory half a microsecond).  A prompt of 8,192 tokens 590 to
+// 670 us with the clock that the card's power allows, 0.72 to 0.82 PFLOP/s; one of 2,048 63 + 9; 512 tokens behind 1,536 39 + 6.
 #include <math.h>
 
 #include "api.h"
@@ -300,8 +300,8 @@ __device__ __forceinline__ float kv4_operands(Kv4Queries<HD>& q, float scale, u3
 // A workgroup has a chunk of a token and a set of up to sixteen query heads of a key head: grid (key heads x sets, work items).  Each of its
 // waves takes every KV4_WAVES-th block; what they sum is joined through LDS, in the order of the waves.  Of a token of one chunk the output
 // is stored at once; else output, reference and sum go to `partial` ([slot][head][chunk][HD], then [slot][head][chunk][2]).
-// Bound by the cache's bytes where there is work for the chip (three workgroups of 12 waves a CU have 110 KB of it on their way), by dependent trips
-// to memory where there is not.
+// Bound by the cache's bytes where there is work for the chip (three workgroups of 12 waves a CU have 110 KB of it on their way), by
+// dependent trips to memory where there is not.
 template <int HD>
 __global__ void __launch_bounds__(64 * KV4_WAVES, TERMS == 1 ? 3 : 2)
 kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned char* __restrict__ k_cache,
@@ -416,8 +416,8 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
 }
 
 // A token's chunks joined: with M the largest of their maxima, out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M); JOIN_SUMS sums side
-// by side over every JOIN_SUMS-th chunk, ascending, added in order.  grid (tokens, heads); a thread has four dims of one of the sums.  Bound by its
-// launch: 3.3 us for one token of 9 chunks, 4.0 for 64, 7.6 for 8 of 128 chunks.
+// by side over every JOIN_SUMS-th chunk, ascending, added in order.  grid (tokens, heads); a thread has four dims of one of the sums. 
+// Bound by its launch: 3.3 us for one token of 9 chunks, 4.0 for 64, 7.6 for 8 of 128 chunks.
 #define JOIN_SUMS 8
 template <int HD>
 __global__ void __launch_bounds__(JOIN_SUMS * HD / 4)
@@ -484,23 +484,23 @@ kv4_join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ p
 
 // ============================================================================ prompt portions
 // A workgroup has a tile of up to 128 consecutive tokens of one request and HPB query heads of a key head, four waves a head, 32 rows each;
-// grid (key heads x sets of HPB heads, tiles), tiles with the most work first, so that the shortest are left for the end.  A block of 64 positions is unpacked once a workgroup, an octet of slots a
-// wave, into half precision in LDS, where all waves read it: K [64][HD] and V^T [HD][64], 16-byte pieces of a row permuted so that
-// sixteen neighbouring rows' pieces lie in different banks.  Two stages: block b + 1 is unpacked, and block b + 2 on its way in registers
-// (four and a half bits a number, so few), beside the products of block b.
-// S^T = K Q^T and O^T = V^T P^T by 32x32x16 products: what a lane holds of the first is its operand of the second.  Row r of a tile
-// of S^T is position pi(r) of it, pi swapping bits 2 and 3, so that register e of tile pt is position 32 pt + 16 (e / 8) + 8 half + e % 8.
-// Of a block a wave has 32 products (1,024 cycles of its matrix core), 235 vector instructions, 32 of them exponentials, and 32 KB of LDS to read: of a prompt
-// of 8,192 tokens the matrix cores are at work for 42 % of the cycles, the vector units for 57 %, LDS for some 55 %, at the 1.8 GHz that
-// the card's power allows then.  A tile alone takes 1.5 us a block.
+// grid (key heads x sets of HPB heads, tiles), tiles with the most work first, so that the shortest are left for the end.  A block of 64
+// positions is unpacked once a workgroup, an octet of slots a wave, into half precision in LDS, where all waves read it: K [64][HD] and V^T
+// [HD][64], 16-byte pieces of a row permuted so that sixteen neighbouring rows' pieces lie in different banks.  Two stages: block b + 1 is
+// unpacked, and block b + 2 on its way in registers (four and a half bits a number, so few), beside the products of block b. S^T = K Q^T
+// and O^T = V^T P^T by 32x32x16 products: what a lane holds of the first is its operand of the second.  Row r of a tile of S^T is position
+// pi(r) of it, pi swapping bits 2 and 3, so that register e of tile pt is position 32 pt + 16 (e / 8) + 8 half + e % 8. Of a block a wave
+// has 32 products (1,024 cycles of its matrix core), 235 vector instructions, 32 of them exponentials, and 32 KB of LDS to read: of a
+// prompt of 8,192 tokens the matrix cores are at work for 42 % of the cycles, the vector units for 57 %, LDS for some 55 %, at the 1.8 GHz
+// that the card's power allows then.  A tile alone takes 1.5 us a block.
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 #define KV4_ROWS 128               // tokens of a tile
-// Positions lie in segments that end at 1,024, 2,048, 4,096, 8,192 and every 8,192 behind.  What a row sums is closed at a segment's end and folded,
-// in order, into what the segments before gave, whether one workgroup takes them all (its sums then wait in the workspace) or one each, which
-// kv4_fold_kernel joins: the same bits, so a row's result does not depend on how many tiles a step has.  Workgroups that began together
-// get to a segment's end together, and their 128 KB each take 6 us there and 6 back.  With ends at 2,048 and 8,192 alone / these, 28 heads over 4 of 128 dims:
-// 512 tokens behind 1,536 60 / 39 + 6 us, 980 in ragged portions up to 4,400 positions 81 + 5 / 68 + 9, a prompt of 2,048 69 / 63 + 9, of 4,096 179 /
-// 190, of 8,192 670 / 685 (without ends 650; with one every 2,048 700).
+// Positions lie in segments that end at 1,024, 2,048, 4,096, 8,192 and every 8,192 behind.  What a row sums is closed at a segment's end
+// and folded, in order, into what the segments before gave, whether one workgroup takes them all (its sums then wait in the workspace) or
+// one each, which kv4_fold_kernel joins: the same bits, so a row's result does not depend on how many tiles a step has.  Workgroups that
+// began together get to a segment's end together, and their 128 KB each take 6 us there and 6 back.  With ends at 2,048 and 8,192 alone /
+// these, 28 heads over 4 of 128 dims: 512 tokens behind 1,536 60 / 39 + 6 us, 980 in ragged portions up to 4,400 positions 81 + 5 / 68 + 9,
+// a prompt of 2,048 69 / 63 + 9, of 4,096 179 / 190, of 8,192 670 / 685 (without ends 650; with one every 2,048 700).
 #define KV4_MANY 20                // a cut tile's first row names its segment and, from this bit on, how many there are
 __host__ __device__ inline int kv4_segment_of(int p) { return p < 1024 ? 0 : p < 2048 ? 1 : p < 4096 ? 2 : p < 8192 ? 3 : 3 + p / 8192; }
 __host__ __device__ inline int kv4_segment_start(int s) { return s < 3 ? s * 1024 : s == 3 ? 4096 : s > 262146 ? 0x7fffffff : (s - 3) * 8192; }
@@ -570,7 +570,8 @@ __device__ __forceinline__ void kv4_edge(Kv4Octet<HD>& in, int octet, int p, int
 // Unpacked into its stages, as octet `octet` of its block, in PIECES pieces (0, 1: keys, 2, 3: values).
 #define KV4_PIECES 4
 template <int HD>
-__device__ __forceinline__ void kv4_unpack(const Kv4Octet<HD>& in, unsigned char* k_stage, unsigned char* v_stage, int octet, int piece, const Kv4Masks& masks, int lane) {
+__device__ __forceinline__ void kv4_unpack(const Kv4Octet<HD>& in, unsigned char* k_stage, unsigned char* v_stage, int octet, int piece,
+                                           const Kv4Masks& masks, int lane) {
   half2_t sc[4], cc[4];
   const int w = piece & 1;
   if (w >= HD / 64) return;
@@ -789,9 +790,9 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     kv4_meet();
   };
   const int from = live ? max(0, wave_first - base) / KV4_BLOCK : n_blocks, to = live ? min((wave_last - base) / KV4_BLOCK, n_blocks - 1) : -1;
-  // The second head's waves meet the others between a block's scores and its weights: the matrix cores have the products of the one head's scores
-  // while the vector unit has the weights of the other's block before.  (So its values are read while those two blocks on are unpacked.)  Prompts of
-  // 3,600 tokens 160 -> 155 us, of 6,000 412 -> 398; of 8,192, where the card's power bounds it, within 1 %.
+  // The second head's waves meet the others between a block's scores and its weights: the matrix cores have the products of the one head's
+  // scores while the vector unit has the weights of the other's block before.  (So its values are read while those two blocks on are
+  // unpacked.)  Prompts of 3,600 tokens 160 -> 155 us, of 6,000 412 -> 398; of 8,192, where the card's power bounds it, within 1 %.
   const bool late = HPB == 2 && wave >= 4;
   unsigned nan_groups = 0;                         // groups of 32 dims in which the lane's row sees a value that is not a number
   bool kept = false;                               // segments before this one wait in the workspace
@@ -803,8 +804,8 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
     const int p0 = base + b * KV4_BLOCK;
     mend(b + 1);
     {
-      // A row begins at a multiple of its size, and piece 2 n + half of it is piece `half` with n's bits exclusive-ored in: one instruction from a
-      // base each.  The bases are opaque, or the compiler keeps every address in a register across the loop.
+      // A row begins at a multiple of its size, and piece 2 n + half of it is piece `half` with n's bits exclusive-ored in: one instruction
+      // from a base each.  The bases are opaque, or the compiler keeps every address in a register across the loop.
       unsigned k_base = lds0 + k_at(b) + k_row * (HD * 2) + ((half ^ S::k_swizzle(k_row)) << 4);
       unsigned v_base = lds0 + v_at(b) + l32 * 128 + ((half ^ S::v_swizzle(l32)) << 4);
       asm volatile("" : "+v"(k_base), "+v"(v_base));
@@ -874,8 +875,8 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
           for (int e = 0; e < 16; ++e) o[dt][e] = __fmul_rn(o[dt][e], factor);
       }
       const float add = ref == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, ref);
-      // The weights of sixteen positions, then their products with all dims: on those the matrix cores work while the vector unit has the weights
-      // of the next sixteen.
+      // The weights of sixteen positions, then their products with all dims: on those the matrix cores work while the vector unit has the
+      // weights of the next sixteen.
       float sum[2] = {0.0f, 0.0f};
       u32x4 vf[2][DT];
       auto read_v = [&](int st) {
@@ -942,14 +943,15 @@ kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned ch
                             partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);
 }
 
-// The segments of the tiles whose segments had a workgroup each, folded in order: rows that say how many there are, which lie in as many slots from
-// theirs on.  grid (heads, groups of 32 dims, KV4_FOLDS that share the rows); a thread has sixteen dims of a row of the tile, half of the group, as
-// kv4_store left them.  Bound by its launch (2.9 us of one that does nothing) and two trips to memory: 5.6 us for four tiles of two segments
-// of 28 heads of 128 dims, 13 for eight of up to four, 4.7 where nothing was cut.
+// The segments of the tiles whose segments had a workgroup each, folded in order: rows that say how many there are, which lie in as many
+// slots from theirs on.  grid (heads, groups of 32 dims, KV4_FOLDS that share the rows); a thread has sixteen dims of a row of the tile,
+// half of the group, as kv4_store left them.  Bound by its launch (2.9 us of one that does nothing) and two trips to memory: 5.6 us for
+// four tiles of two segments of 28 heads of 128 dims, 13 for eight of up to four, 4.7 where nothing was cut.
 #define KV4_FOLDS 8
 template <int HD>
 __global__ void __launch_bounds__(256)
-kv4_fold_kernel(elem_t* __restrict__ out, const int32_t* __restrict__ tiles, int n_tiles, const float* __restrict__ partial, int n_slots, int n_heads) {
+kv4_fold_kernel(elem_t* __restrict__ out, const int32_t* __restrict__ tiles, int n_tiles, const float* __restrict__ partial, int n_slots,
+                int n_heads) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x, dt = blockIdx.y, my_row = wave * 32 + (lane & 31);
   const size_t tile = (size_t)n_heads * Kv4State<HD>::FLOATS;
   for (int first = 0, seen = 0; first < n_tiles; first += 64) {
@@ -1023,12 +1025,13 @@ extern "C" int axk_kv4_attention_decode(const void* q, int q_stride, const void*
 #undef LAUNCH
   AXK_LAUNCH_CHECK("kv4_attention_decode");
   if (max_chunks > 1) {
-    if (head_dim == 64)
-      kv4_join_kernel<64><<<dim3(n_tokens, n_heads), JOIN_SUMS * 16, 0, (hipStream_t)stream>>>(partial, positions, token_index, (elem_t*)out, n_tokens,
-                                                                                    max_chunks, n_heads, window);
-    else
-      kv4_join_kernel<128><<<dim3(n_tokens, n_heads), JOIN_SUMS * 32, 0, (hipStream_t)stream>>>(partial, positions, token_index, (elem_t*)out,
-                                                                                     n_tokens, max_chunks, n_heads, window);
+    const dim3 rows(n_tokens, n_heads);
+#define JOIN(HD)                                                                                                                \
+  kv4_join_kernel<HD><<<rows, JOIN_SUMS * HD / 4, 0, (hipStream_t)stream>>>(partial, positions, token_index, (elem_t*)out,      \
+                                                                            n_tokens, max_chunks, n_heads, window)
+    if (head_dim == 64) JOIN(64);
+    else JOIN(128);
+#undef JOIN
     AXK_LAUNCH_CHECK("kv4_attention_decode");
   }
   return 0;
@@ -1077,8 +1080,9 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
         positions, seq_rows, (elem_t*)out, tiles, partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);             \
   }
 #if AXON_BF16
-  // One query head a workgroup while there are up to three a CU, which spread better; beyond that two, which share what is unpacked: 672 tiles and
-  // heads in ragged portions 68 against 73 us, 616 of a prompt of 2,800 tokens 103 against 110, 896 of one of 4,096 199 against 190.
+  // One query head a workgroup while there are up to three a CU, which spread better; beyond that two, which share what is unpacked: 672
+  // tiles and heads in ragged portions 68 against 73 us, 616 of a prompt of 2,800 tokens 103 against 110, 896 of one of 4,096 199 against
+  // 190.
   if (group >= 2 && (long)n_tiles * n_heads > 768) {
     if (head_dim == 64) LAUNCH(64, 2) else LAUNCH(128, 2)
   } else

@@ -92,9 +92,9 @@ __device__ inline unsigned kv4_quantise8(const float (&x)[8], unsigned (&n)[8]) 
   return bits | (unsigned)z;
 }
 
-// Dims c0 .. c0 + 7 of a head's row behind the rotation (rotate-half on the first rotary_dim dims; half a multiple of 8).  All loads are without a
-// branch, so that they are under way together: dims that do not turn read themselves and the table's first 64 bytes, which have to be
-// there also where nothing turns.
+// Dims c0 .. c0 + 7 of a head's row behind the rotation (rotate-half on the first rotary_dim dims; half a multiple of 8).  All loads are
+// without a branch, so that they are under way together: dims that do not turn read themselves and the table's first 64 bytes, which have
+// to be there also where nothing turns.
 __device__ inline void rotated8(const elem_t* head, const float* tab, int c0, int rotary_dim, float (&out)[8]) {
   const int half = rotary_dim / 2, to = c0 >= half ? -half : half;
   const bool turn = c0 < rotary_dim, upper = c0 >= half;
@@ -113,11 +113,11 @@ __device__ inline void rotated8(const elem_t* head, const float* tab, int c0, in
   }
 }
 
-// The blocks behind the first kv_blocks have the queries of Q_TOKENS tokens each: a thread the eight pairs of dims i .. i + 7 and i + half .. (or
-// sixteen dims behind the rotated ones) of several heads of a token, whose sines and cosines it reads once.  The first, which take longer, have the keys and
-// values of up to `rows` tokens: a thread a word of keys, or eight dims of a run's values, whose words hold up to eight positions.
-// Bound by its bytes in prompts (qkv in, q and the cache out: 8192 tokens of 28 and 4 heads of 128 dims take 25 us, 143 MB at 5.7 TB/s), by its waits
-// in steps of few tokens (8: 4.8 us; a launch of the queries' blocks alone 2.9).
+// The blocks behind the first kv_blocks have the queries of Q_TOKENS tokens each: a thread the eight pairs of dims i .. i + 7 and i + half
+// .. (or sixteen dims behind the rotated ones) of several heads of a token, whose sines and cosines it reads once.  The first, which take
+// longer, have the keys and values of up to `rows` tokens: a thread a word of keys, or eight dims of a run's values, whose words hold up to
+// eight positions. Bound by its bytes in prompts (qkv in, q and the cache out: 8192 tokens of 28 and 4 heads of 128 dims take 25 us, 143 MB
+// at 5.7 TB/s), by its waits in steps of few tokens (8: 4.8 us; a launch of the queries' blocks alone 2.9).
 template <int Q_TOKENS>
 __global__ void __launch_bounds__(256)
 rope_kv4_write_kernel(const elem_t* qkv, long qkv_stride, elem_t* q_out, long q_stride, const float* __restrict__ table,
@@ -260,16 +260,19 @@ extern "C" int axk_rope_kv4_write(const void* qkv, long qkv_stride, void* q_out,
   AXK_REQUIRE(!write_kv || ((uintptr_t)k_cache % 16 == 0 && (uintptr_t)v_cache % 16 == 0), "rope_kv4_write: caches must be 16-byte aligned");
   AXK_REQUIRE((uintptr_t)table % 16 == 0, "rope_kv4_write: the table must be 16-byte aligned");
   if (n_tokens == 0) return 0;
-  // Few tokens: a block each for its queries and for its keys and values.  Of 28 query and 4 key/value heads of 128 dims, so or in blocks of four
-  // and eight tokens: 8 single tokens 4.7 and 9.4 us, 128 7.7 and 12.9, 512 17.9 and 21.1; a portion of 64 tokens 7.2 and 9.1, of 1024 9.6 and
-  // 10.9, of 2048 16.6 and 13.2.  Blocks of sixteen tokens: 1024 13.4, 4096 17.4 against 17.1 by eight, 8192 24.8 against 26.7.
+  // Few tokens: a block each for its queries and for its keys and values.  Of 28 query and 4 key/value heads of 128 dims, so or in blocks
+  // of four and eight tokens: 8 single tokens 4.7 and 9.4 us, 128 7.7 and 12.9, 512 17.9 and 21.1; a portion of 64 tokens 7.2 and 9.1, of
+  // 1024 9.6 and 10.9, of 2048 16.6 and 13.2.  Blocks of sixteen tokens: 1024 13.4, 4096 17.4 against 17.1 by eight, 8192 24.8 against
+  // 26.7.
   const bool few = n_tokens <= 1024;
-  const int rows = few ? 1 : n_tokens <= 4096 ? 8 : LIST_ROWS, q_blocks = few ? n_tokens : ceil_div(n_tokens, 4), kv_blocks = write_kv ? ceil_div(n_tokens, rows) : 0;
+  const int rows = few ? 1 : n_tokens <= 4096 ? 8 : LIST_ROWS, q_blocks = few ? n_tokens : ceil_div(n_tokens, 4);
+  const int kv_blocks = write_kv ? ceil_div(n_tokens, rows) : 0;
   const unsigned blocks = q_blocks + kv_blocks;
 #define LAUNCH(Q_TOKENS)                                                                                                          \
   rope_kv4_write_kernel<Q_TOKENS><<<blocks, 256, 0, (hipStream_t)stream>>>(                                                       \
-      (const elem_t*)qkv, qkv_stride, (elem_t*)q_out, q_stride, rotary_dim > 0 ? table : (const float*)qkv, positions, seq_rows, block_table, table_stride,            \
-      (unsigned char*)k_cache, (unsigned char*)v_cache, n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, page_size, kv_blocks, rows)
+      (const elem_t*)qkv, qkv_stride, (elem_t*)q_out, q_stride, rotary_dim > 0 ? table : (const float*)qkv, positions, seq_rows,  \
+      block_table, table_stride, (unsigned char*)k_cache, (unsigned char*)v_cache, n_tokens, n_heads, n_kv_heads, head_dim,       \
+      rotary_dim, page_size, kv_blocks, rows)
   if (few) LAUNCH(1);
   else LAUNCH(4);
 #undef LAUNCH
@@ -280,8 +283,8 @@ extern "C" int axk_rope_kv4_write(const void* qkv, long qkv_stride, void* q_out,
 // Rows (seq_rows[i], positions[i]) of the cache as plain rows [n][kv heads][head_dim] of the compute dtype, each number rounded
 // once (bfloat16 holds eight of its up to ten bits).  grid (lists of LIST_ROWS rows, keys | values): a thread a word of keys, or the words of
 // eight dims of a run's values, which it unpacks as the products' operands are.  A run of whole octets is its
-// first block's; no words are read twice.  Bound by the rows that it stores: eight requests' 16384 positions of 4 heads of 128 dims take 80 us, 344 MB at 4.3 TB/s;
-// by its waits for few (301 rows: 4.7 us).
+// first block's; no words are read twice.  Bound by the rows that it stores: eight requests' 16384 positions of 4 heads of 128 dims take 76
+// us, 344 MB at 4.5 TB/s; by its waits for few (301 rows: 4.5 us).
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const unsigned char* __restrict__ k_cache, const unsigned char* __restrict__ v_cache,
                 const int32_t* __restrict__ block_table, int table_stride, const int32_t* __restrict__ positions,
