@@ -38,6 +38,8 @@ def ptr(t: Optional[torch.Tensor]) -> c_void_p:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 
 
 def _stream() -> c_void_p:
@@ -1685,25 +1687,28 @@ class Kernels:
         """Bytes of a position's keys (or values) of one head, its scales among them."""
         return int(self.run.axk_kv4_row_bytes(head_dim))
 
-    def _kv4_step(self, what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, *others) -> int:
-        """The checks that the 4-bit cache's calls share; the number of tokens."""
-        # (in few calls of torch: these run before every launch of a step that takes some 10 us; a tensor of the host is on device -1)
+    def _kv4_step(self, what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, *others):
+        """The checks that the 4-bit cache's calls share; (number of tokens, the current stream)."""
+        # (in few and short calls of torch: these run before every launch of a step that takes some 10 us; a tensor of the host is on device -1)
         row = self._kv4_bytes.get((head_dim, page_size))
         if row is None:
             row = self._kv4_bytes[head_dim, page_size] = self.kv4_row_bytes(head_dim) if self.kv4_ok(head_dim, page_size) else 0
         if row == 0:
             raise KernelError(f"{what}: head_dim {head_dim} and pages of {page_size} positions are not taken by the 4-bit cache")
-        here = torch.cuda.current_device() if _raw_stream is None else torch._C._cuda_getDevice()
-        for t in (positions, seq_rows, block_table):
-            if t.dtype is not torch.int32 or t.get_device() != here or not t.is_contiguous():
-                raise KernelError(f"{what}: expected contiguous int32 tensors on cuda:{here}, got {t.dtype} on {t.device}")
-        if positions.dim() != 1 or seq_rows.shape != positions.shape or block_table.dim() != 2:
+        here = _device()
+        if (positions.dtype is not _I32 or seq_rows.dtype is not _I32 or block_table.dtype is not _I32 or positions.get_device() != here
+                or seq_rows.get_device() != here or block_table.get_device() != here or not positions.is_contiguous()
+                or not seq_rows.is_contiguous() or not block_table.is_contiguous()):
+            raise KernelError(f"{what}: expected contiguous int32 tensors on cuda:{here}, got " +
+                              ", ".join(f"{t.dtype} on {t.device}" for t in (positions, seq_rows, block_table)))
+        T = positions.numel()
+        if positions.dim() != 1 or seq_rows.dim() != 1 or seq_rows.numel() != T or block_table.dim() != 2:
             raise KernelError(f"{what}: positions {tuple(positions.shape)}, seq_rows {tuple(seq_rows.shape)}, block_table {tuple(block_table.shape)}")
         if k_cache is not None:
             shape = k_cache.shape
-            if (shape[1:] != (n_kv_heads, page_size, row) or v_cache.shape != shape or k_cache.dtype is not torch.uint8
-                    or v_cache.dtype is not torch.uint8 or not k_cache.is_contiguous() or not v_cache.is_contiguous()
-                    or k_cache.get_device() != here or v_cache.get_device() != here):
+            if (len(shape) != 4 or shape != (shape[0], n_kv_heads, page_size, row) or v_cache.shape != shape or k_cache.dtype is not _U8
+                    or v_cache.dtype is not _U8 or k_cache.get_device() != here or v_cache.get_device() != here
+                    or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
                 raise KernelError(f"{what}: caches {tuple(shape)} and {tuple(v_cache.shape)} of {k_cache.dtype} and {v_cache.dtype} on {k_cache.device} "
                                   f"and {v_cache.device} are not uint8 [pages, {n_kv_heads}, {page_size}, {row}] on cuda:{here}")
             if k_cache.numel() > 1 << 37:                        # places in it are 32-bit numbers of 32 bytes
@@ -1711,7 +1716,7 @@ class Kernels:
         for t in others:
             if t.get_device() != here:
                 raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
-        return positions.numel()
+        return T, (_queue() if _raw_stream is None else _raw_stream(here))
 
     def rope_kv4_write(self, qkv, q_out, table, positions, seq_rows, block_table, k_cache, v_cache, n_heads, n_kv_heads, head_dim,
                        rotary_dim, page_size, write_kv=True) -> None:
@@ -1719,8 +1724,10 @@ class Kernels:
         k head of qkv [T, (n_heads + 2 n_kv_heads) head_dim], whose rows may lie apart; q to q_out [T, n_heads head_dim] (qkv's own
         columns are allowed), k and v quantised from 32 bits into the pages; a request's position is there once in a step (of two that are
         the same neither may be what is held).  Without write_kv, q alone."""
-        self._elem(qkv, "rope qkv"); self._elem(q_out, "rope q"); self._f32(table, "rope table")
-        T = self._kv4_step("rope_kv4_write", k_cache if write_kv else None, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim,
+        if qkv.dtype is not self.dtype or q_out.dtype is not self.dtype or table.dtype is not _F32 or not table.is_contiguous():
+            raise KernelError(f"rope_kv4_write: qkv and q_out of {qkv.dtype} and {q_out.dtype}, a table of {table.dtype}: expected {self.dtype_name} "
+                              "and contiguous float32")
+        T, stream = self._kv4_step("rope_kv4_write", k_cache if write_kv else None, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim,
                            page_size, qkv, q_out, table)
         width = (n_heads + (2 * n_kv_heads if write_kv else 0)) * head_dim
         if qkv.dim() != 2 or qkv.shape[0] != T or qkv.shape[1] < width or qkv.stride(1) != 1:
@@ -1729,21 +1736,27 @@ class Kernels:
             raise KernelError(f"rope_kv4_write: q_out {tuple(q_out.shape)} is not [{T}, {n_heads * head_dim}]")
         if table.shape != (T, rotary_dim // 2, 2):
             raise KernelError(f"rope_kv4_write: table {tuple(table.shape)} for rotary_dim {rotary_dim}")
-        self._check(self.run.axk_rope_kv4_write(
-            _ptr(qkv), qkv.stride(0), _ptr(q_out), q_out.stride(0), _ptr(table), _ptr(positions), _ptr(seq_rows), _ptr(block_table),
-            block_table.shape[-1], _ptr(k_cache if write_kv else None), _ptr(v_cache if write_kv else None), T, n_heads, n_kv_heads,
-            head_dim, rotary_dim, page_size, 1 if write_kv else 0, _queue()))
+        rc = self.run.axk_rope_kv4_write(
+            qkv.data_ptr(), qkv.stride(0), q_out.data_ptr(), q_out.stride(0), table.data_ptr(), positions.data_ptr(), seq_rows.data_ptr(),
+            block_table.data_ptr(), block_table.shape[1], k_cache.data_ptr() if write_kv else None, v_cache.data_ptr() if write_kv else None,
+            T, n_heads, n_kv_heads, head_dim, rotary_dim, page_size, 1 if write_kv else 0, stream)
+        if rc != 0:
+            self._check(rc)
 
     def kv4_read(self, k_cache, v_cache, block_table, positions, seq_rows, k_out, v_out, n_kv_heads, head_dim, page_size) -> None:
         """The rows of (seq_rows[i], positions[i]) out of a cache held in 4 bits: k_out, v_out [n, n_kv_heads, head_dim] of the
         compute dtype, each number rounded once."""
-        self._elem(k_out, "kv4_read k"); self._elem(v_out, "kv4_read v")
-        n = self._kv4_step("kv4_read", k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, k_out, v_out)
-        for out in (k_out, v_out):
-            if out.shape != (n, n_kv_heads, head_dim) or not out.is_contiguous():
-                raise KernelError(f"kv4_read: rows {tuple(out.shape)} are not [{n}, {n_kv_heads}, {head_dim}]")
-        self._check(self.run.axk_kv4_read(_ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[-1], _ptr(positions),
-                                          _ptr(seq_rows), _ptr(k_out), _ptr(v_out), n, n_kv_heads, head_dim, page_size, _queue()))
+        n, stream = self._kv4_step("kv4_read", k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, k_out,
+                                   v_out)
+        shape, dtype = (n, n_kv_heads, head_dim), self.dtype
+        if (k_out.shape != shape or v_out.shape != shape or k_out.dtype is not dtype or v_out.dtype is not dtype or not k_out.is_contiguous()
+                or not v_out.is_contiguous()):
+            raise KernelError(f"kv4_read: rows {tuple(k_out.shape)} of {k_out.dtype} and {tuple(v_out.shape)} of {v_out.dtype} are not {list(shape)} "
+                              f"of {self.dtype_name}")
+        rc = self.run.axk_kv4_read(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], positions.data_ptr(),
+                                   seq_rows.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), n, n_kv_heads, head_dim, page_size, stream)
+        if rc != 0:
+            self._check(rc)
 
     def _kv4_chunk_sizes(self, seen):
         """Positions of a chunk for tokens that see so many (the kernel's rule: it grows with them, up to its largest)."""
@@ -1800,12 +1813,12 @@ class Kernels:
         return int(self.run.axk_kv4_decode_workspace(n_tokens, n_heads, head_dim, max_chunks))
 
     def _kv4_rows(self, what, q, q_stride, out, T, n_heads, head_dim) -> None:
-        width = n_heads * head_dim
-        if q.dtype is not self.dtype or q.dim() < 1 or q.stride(-1) != 1:
+        width, dtype = n_heads * head_dim, self.dtype
+        if q.dtype is not dtype or q.stride()[-1:] != (1,):
             raise KernelError(f"{what}: q {tuple(q.shape)} of {q.dtype} is not rows of {self.dtype_name}")
         if T > 0 and (q_stride < width or not self._holds(q, (T - 1) * q_stride + width)):
             raise KernelError(f"{what}: rows {q_stride} apart of q {tuple(q.shape)} do not hold {T} rows of {n_heads} heads of {head_dim}")
-        if out.dtype is not self.dtype or out.shape != (T, width) or not out.is_contiguous():
+        if out.dtype is not dtype or out.shape != (T, width) or not out.is_contiguous():
             raise KernelError(f"{what}: out {tuple(out.shape)} of {out.dtype} is not [{T}, {width}] of {self.dtype_name}")
 
     @staticmethod
@@ -1818,25 +1831,28 @@ class Kernels:
         """`attention_decode` over a cache held in 4 bits: tokens named by token_index (int32), or the first `token_index` of the
         step.  `work` (int32, on the device): `kv4_decode_work` of their positions, -1 for nothing; partial: float32,
         `kv4_decode_workspace`."""
-        T = self._kv4_step("kv4_attention_decode", k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size,
-                           q, out, partial, work)
-        self._kv4_rows("kv4_attention_decode", q, q_stride, out, T, n_heads, head_dim)
+        what = "kv4_attention_decode"
+        T, stream = self._kv4_step(what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, q, out, partial,
+                                   work)
+        self._kv4_rows(what, q, q_stride, out, T, n_heads, head_dim)
         if isinstance(token_index, int):
-            n, token_index = token_index, None
+            n, index = token_index, None
         else:
             self._i32(token_index, "token_index")
-            n = token_index.numel()
-        self._f32(partial, "attention partial"); self._i32(work, "attention work list")
+            n, index = token_index.numel(), token_index.data_ptr()
+        if partial.dtype is not _F32 or not partial.is_contiguous() or work.dtype is not _I32 or not work.is_contiguous() or work.dim() != 1:
+            raise KernelError(f"{what}: a workspace of {partial.dtype}, a work list {tuple(work.shape)} of {work.dtype}: expected contiguous float32 "
+                              "and int32")
         if not 0 <= n <= T:
-            raise KernelError(f"kv4_attention_decode: {n} tokens of a step of {T}")
-        if max_chunks < 1 or partial.numel() < self.kv4_decode_workspace(n, n_heads, head_dim, max_chunks):
-            raise KernelError(f"kv4_attention_decode: workspace of {partial.numel()} floats is too small for {max_chunks} chunks")
-        if work.dim() != 1:
-            raise KernelError(f"kv4_attention_decode: work list {tuple(work.shape)}")
-        self._check(self.run.axk_kv4_attention_decode(
-            _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[-1], _ptr(positions), _ptr(seq_rows),
-            _ptr(out), _ptr(token_index), n, _ptr(work), work.numel(), _ptr(partial), max_chunks, n_heads, n_kv_heads, head_dim,
-            page_size, window, float(scale), _queue()))
+            raise KernelError(f"{what}: {n} tokens of a step of {T}")
+        if max_chunks < 1 or partial.numel() < self.run.axk_kv4_decode_workspace(n, n_heads, head_dim, max_chunks):
+            raise KernelError(f"{what}: workspace of {partial.numel()} floats is too small for {max_chunks} chunks")
+        rc = self.run.axk_kv4_attention_decode(
+            q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], positions.data_ptr(),
+            seq_rows.data_ptr(), out.data_ptr(), index, n, work.data_ptr(), work.numel(), partial.data_ptr(), max_chunks, n_heads, n_kv_heads,
+            head_dim, page_size, window, float(scale), stream)
+        if rc != 0:
+            self._check(rc)
         return out
 
     def kv4_prefill_tiles(self, spans, window: int, n_heads: int, n_kv_heads: int) -> List[tuple]:
@@ -1879,16 +1895,20 @@ class Kernels:
                               n_kv_heads, head_dim, page_size, window, scale) -> torch.Tensor:
         """`attention_prefill` over a cache held in 4 bits: prompt portions by `kv4_prefill_tiles` (int32 [n, 4] on the device); partial:
         float32, `kv4_prefill_workspace` of these tiles.  Rows of no tile are left as they are."""
-        T = self._kv4_step("kv4_attention_prefill", k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size,
-                           q, out, tiles, partial)
-        self._kv4_rows("kv4_attention_prefill", q, q_stride, out, T, n_heads, head_dim)
-        self._i32(tiles, "tiles"); self._f32(partial, "attention partial")
+        what = "kv4_attention_prefill"
+        T, stream = self._kv4_step(what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, q, out, tiles,
+                                   partial)
+        self._kv4_rows(what, q, q_stride, out, T, n_heads, head_dim)
+        if partial.dtype is not _F32 or not partial.is_contiguous() or tiles.dtype is not _I32 or not tiles.is_contiguous():
+            raise KernelError(f"{what}: a workspace of {partial.dtype}, tiles of {tiles.dtype}: expected contiguous float32 and int32")
         if tiles.numel() and (tiles.dim() != 2 or tiles.shape[1] != 4):
-            raise KernelError(f"kv4_attention_prefill: tiles {tuple(tiles.shape)}")
-        self._check(self.run.axk_kv4_attention_prefill(
-            _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[-1], _ptr(positions), _ptr(seq_rows),
-            _ptr(out), _ptr(tiles), tiles.numel() // 4, _ptr(partial), partial.numel(), n_heads, n_kv_heads, head_dim, page_size, window,
-            float(scale), _queue()))
+            raise KernelError(f"{what}: tiles {tuple(tiles.shape)}")
+        rc = self.run.axk_kv4_attention_prefill(
+            q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], positions.data_ptr(),
+            seq_rows.data_ptr(), out.data_ptr(), tiles.data_ptr(), tiles.numel() // 4, partial.data_ptr(), partial.numel(), n_heads, n_kv_heads,
+            head_dim, page_size, window, float(scale), stream)
+        if rc != 0:
+            self._check(rc)
         return out
 
     def fill_i32(self, dst: torch.Tensor, value: int) -> None:
