@@ -536,20 +536,19 @@ int axk_kv4_attention_decode(const void* q, int q_stride, const void* k_cache, c
                              const int32_t* token_index, int n_tokens, const int32_t* work, int n_work, float* partial,
                              int max_chunks, int n_heads, int n_kv_heads, int head_dim, int page_size, int window, float scale,
                              void* stream);
-// Prompt portions: tiles [n_tiles][4] = (first token, count up to axk_kv4_prefill_tile, segment, slot).  segment -1: everything that the
-// tile's rows see, which needs a slot of the workspace (its own, else -1) if that lies in several segments of positions
-// (axk_kv4_prefill_segment); segment s: only the positions from axk_kv4_prefill_segment_start(s) up to the next, into its slot.  A tile that is
-// cut has a row for each of its n segments, their slots in order, of which the first says n << axk_kv4_prefill_many() | s: a second
-// launch folds them into the tile's rows of out.  The same bits either way.
-int axk_kv4_prefill_many(void);
+// Prompt portions: tiles [n_tiles][columns] = (first token, count up to axk_kv4_prefill_tile, segment, slot[, segments]).  segment -1:
+// everything that the tile's rows see, which needs a slot of the workspace (its own, else -1) if that lies in several segments of
+// positions (axk_kv4_prefill_segment); segment s: only the positions from axk_kv4_prefill_segment_start(s) up to the next, into its slot.
+// A tile that is cut has a row for each of its segments, their slots in order, of which the first has their number in a fifth column (else 0;
+// 4 columns: no tile is cut): a second launch folds them into the tile's rows of out.  The same bits either way.
 int axk_kv4_prefill_tile(void);
 int axk_kv4_prefill_segment(int position);
 int axk_kv4_prefill_segment_start(int segment);
 long axk_kv4_prefill_workspace(int n_slots, int n_heads, int head_dim);
 int axk_kv4_attention_prefill(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int32_t* block_table,
                               int table_stride, const int32_t* positions, const int32_t* seq_rows, void* out, const int32_t* tiles,
-                              int n_tiles, float* partial, long partial_floats, int n_heads, int n_kv_heads, int head_dim, int page_size,
-                              int window, float scale, void* stream);
+                              int n_tiles, int columns, float* partial, long partial_floats, int n_heads, int n_kv_heads, int head_dim,
+                              int page_size, int window, float scale, void* stream);
 
 #ifdef __cplusplus
 }

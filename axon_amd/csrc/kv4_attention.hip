@@ -500,8 +500,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 // one each, which kv4_fold_kernel joins: the same bits, so a row's result does not depend on how many tiles a step has.  Workgroups that
 // began together get to a segment's end together, and their 128 KB each take 6 us there and 6 back.  With ends at 2,048 and 8,192 alone /
 // these, 28 heads over 4 of 128 dims: 512 tokens behind 1,536 60 / 39 + 6 us, 980 in ragged portions up to 4,400 positions 81 + 5 / 68 + 9,
-// a prompt of 2,048 69 / 63 + 9, of 4,096 179 / 190, of 8,192 670 / 685 (without ends 650; with one every 2,048 700).
-#define KV4_MANY 20                // a cut tile's first row names its segment and, from this bit on, how many there are
+// a prompt of 2,048 69 / 63 + 9, of 4,096 179 / 183, of 8,192 660 / 675 (without ends 650; with one every 2,048 700).
 __host__ __device__ inline int kv4_segment_of(int p) { return p < 1024 ? 0 : p < 2048 ? 1 : p < 4096 ? 2 : p < 8192 ? 3 : 3 + p / 8192; }
 __host__ __device__ inline int kv4_segment_start(int s) { return s < 3 ? s * 1024 : s == 3 ? 4096 : s > 262146 ? 0x7fffffff : (s - 3) * 8192; }
 
@@ -927,26 +926,26 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   kv4_store_row<HD>(st, out_row, lane, nan_groups);
 }
 
-// tiles [n][4] = (first token, count, segment or -1 for all that the tile sees, slot of the workspace).
+// tiles [n][columns] = (first token, count, segment or -1 for all that the tile sees, slot of the workspace, kv4_fold_kernel's).
 template <int HD, int HPB>
 __global__ void __launch_bounds__(256 * HPB, TERMS == 1 ? 2 : 1)
 kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned char* __restrict__ k_cache,
                    const unsigned char* __restrict__ v_cache, const int32_t* __restrict__ block_table, int table_stride,
                    const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows, elem_t* __restrict__ out,
-                   const int32_t* __restrict__ tiles, float* __restrict__ partial, int n_slots, int n_heads, int n_kv_heads, int page_size,
-                   int window, float scale) {
+                   const int32_t* __restrict__ tiles, int columns, float* __restrict__ partial, int n_slots, int n_heads, int n_kv_heads,
+                   int page_size, int window, float scale) {
   extern __shared__ __align__(256) unsigned char smem[];
-  const int32_t* mine = tiles + 4 * blockIdx.y;
-  const int t0 = mine[0], count = mine[1], segment = mine[2] < 0 ? mine[2] : mine[2] & ((1 << KV4_MANY) - 1), slot = mine[3];
+  const int32_t* mine = tiles + columns * blockIdx.y;
+  const int t0 = mine[0], count = mine[1], segment = mine[2], slot = mine[3];
   if (count <= 0 || count > KV4_ROWS || segment < -1) return;
   kv4_prefill_tile<HD, HPB>(smem, t0, count, q, q_stride, k_cache, v_cache, block_table, table_stride, positions, seq_rows, out, segment, slot,
                             partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);
 }
 
-// The segments of the tiles whose segments had a workgroup each, folded in order: rows that say how many there are, which lie in as many
-// slots from theirs on.  grid (heads, groups of 32 dims, KV4_FOLDS that share the rows); a thread has sixteen dims of a row of the tile,
+// The segments of the tiles whose segments had a workgroup each, folded in order: rows of five whose last says how many there are, which lie
+// in as many slots from theirs on.  grid (heads, groups of 32 dims, KV4_FOLDS that share the rows); a thread has sixteen dims of a row of the tile,
 // half of the group, as kv4_store left them.  Bound by its launch (2.9 us of one that does nothing) and two trips to memory: 5.6 us for
-// four tiles of two segments of 28 heads of 128 dims, 13 for eight of up to four, 4.7 where nothing was cut.
+// four tiles of two segments of 28 heads of 128 dims, 13 for eight of up to four.
 #define KV4_FOLDS 8
 template <int HD>
 __global__ void __launch_bounds__(256)
@@ -955,11 +954,11 @@ kv4_fold_kernel(elem_t* __restrict__ out, const int32_t* __restrict__ tiles, int
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.x, dt = blockIdx.y, my_row = wave * 32 + (lane & 31);
   const size_t tile = (size_t)n_heads * Kv4State<HD>::FLOATS;
   for (int first = 0, seen = 0; first < n_tiles; first += 64) {
-    uint64_t folds = __ballot(first + lane < n_tiles && tiles[4 * (first + lane) + 2] >> KV4_MANY > 0);
+    uint64_t folds = __ballot(first + lane < n_tiles && tiles[5 * (first + lane) + 4] > 0);
     for (; folds != 0; folds &= folds - 1) {
       if (seen++ % KV4_FOLDS != (int)blockIdx.z) continue;
-      const int32_t* mine = tiles + 4 * (first + __builtin_ctzll(folds));
-      const int t0 = mine[0], count = mine[1], segments = mine[2] >> KV4_MANY, slot = mine[3];
+      const int32_t* mine = tiles + 5 * (first + __builtin_ctzll(folds));
+      const int t0 = mine[0], count = mine[1], slot = mine[3], segments = mine[4];
       if (count <= 0 || count > KV4_ROWS || slot < 0 || slot > n_slots - segments || wave * 32 >= count) continue;
       const float* at = partial + slot * tile + (size_t)head * Kv4State<HD>::FLOATS;
       Kv4State<32> st;
@@ -1037,7 +1036,6 @@ extern "C" int axk_kv4_attention_decode(const void* q, int q_stride, const void*
   return 0;
 }
 
-extern "C" int axk_kv4_prefill_many(void) { return KV4_MANY; }
 extern "C" int axk_kv4_prefill_segment(int position) { return kv4_segment_of(position); }
 extern "C" int axk_kv4_prefill_segment_start(int segment) { return kv4_segment_start(segment); }
 
@@ -1048,13 +1046,14 @@ extern "C" long axk_kv4_prefill_workspace(int n_slots, int n_heads, int head_dim
 
 extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void* k_cache, const void* v_cache,
                                          const int32_t* block_table, int table_stride, const int32_t* positions,
-                                         const int32_t* seq_rows, void* out, const int32_t* tiles, int n_tiles, float* partial,
-                                         long partial_floats, int n_heads, int n_kv_heads, int head_dim, int page_size, int window,
+                                         const int32_t* seq_rows, void* out, const int32_t* tiles, int n_tiles, int columns,
+                                         float* partial, long partial_floats, int n_heads, int n_kv_heads, int head_dim, int page_size, int window,
                                          float scale, void* stream) {
   const int rc = kv4_attention_args("kv4_attention_prefill", q, q_stride, k_cache, v_cache, out, n_heads, n_kv_heads, head_dim,
                                     page_size, window, scale);
   if (rc != 0) return rc;
   AXK_REQUIRE(n_tiles >= 0 && n_tiles <= 65535 && (n_tiles == 0 || tiles != nullptr), "kv4_attention_prefill: %d tiles (at most 65535)", n_tiles);
+  AXK_REQUIRE(columns == 4 || columns == 5, "kv4_attention_prefill: tiles of %d numbers (4, or 5 where some are cut)", columns);
   AXK_REQUIRE(partial_floats >= 0 && (uintptr_t)partial % 16 == 0 && (partial_floats == 0 || partial != nullptr),
               "kv4_attention_prefill: a workspace of %ld floats, 16-byte aligned", partial_floats);
   if (n_tiles == 0) return 0;
@@ -1077,7 +1076,7 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
     configured |= 1ull << (device & 63);                                                                                        \
     kv4_prefill_kernel<HD, HPB><<<dim3(n_kv_heads * ((group + HPB - 1) / HPB), n_tiles), 256 * HPB, lds, (hipStream_t)stream>>>( \
         (const elem_t*)q, q_stride, (const unsigned char*)k_cache, (const unsigned char*)v_cache, block_table, table_stride,    \
-        positions, seq_rows, (elem_t*)out, tiles, partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);             \
+        positions, seq_rows, (elem_t*)out, tiles, columns, partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);    \
   }
 #if AXON_BF16
   // One query head a workgroup while there are up to three a CU, which spread better; beyond that two, which share what is unpacked: 672
@@ -1092,7 +1091,7 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
   }
 #undef LAUNCH
   AXK_LAUNCH_CHECK("kv4_attention_prefill");
-  if (n_slots > 0) {
+  if (columns == 5 && n_slots > 0) {
     const dim3 folds(n_heads, head_dim / 32, KV4_FOLDS);
     if (head_dim == 64) kv4_fold_kernel<64><<<folds, 256, 0, (hipStream_t)stream>>>((elem_t*)out, tiles, n_tiles, partial, n_slots, n_heads);
     else kv4_fold_kernel<128><<<folds, 256, 0, (hipStream_t)stream>>>((elem_t*)out, tiles, n_tiles, partial, n_slots, n_heads);

@@ -186,7 +186,7 @@ _SIGNATURES = {
     "axk_kv4_attention_decode": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                  c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
     "axk_kv4_attention_prefill": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                                  c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
+                                  c_int, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
 }
 
 
@@ -194,7 +194,7 @@ _SIGNATURES = {
 _PLAIN = ["axk_argmax_workspace", "axk_attention_decode_chunk", "axk_attention_decode_item_factor", "axk_attention_decode_workspace",
           "axk_attention_prefill_tile", "axk_delta_chunked_workspace", "axk_gemm_workspace", "axk_latent_attention_workspace",
           "axk_masked_attention_workspace", "axk_packed_elems", "axk_kv4_decode_chunk", "axk_kv4_decode_item_factor",
-          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile", "axk_kv4_prefill_many", "axk_kv4_prefill_segment",
+          "axk_kv4_decode_workspace", "axk_kv4_prefill_tile", "axk_kv4_prefill_segment",
           "axk_kv4_prefill_segment_start", "axk_kv4_prefill_workspace"]
 
 
@@ -1858,9 +1858,9 @@ class Kernels:
     def kv4_prefill_tiles(self, spans, window: int, n_heads: int, n_kv_heads: int) -> List[tuple]:
         """The tiles of `kv4_attention_prefill` for portions (first token of the step, tokens, position of the first): rows of (first
         token, count, segment, slot of the workspace), those with the most work first.  A tile whose rows see several segments of positions is
-        cut there where a step has few tiles (its segments then run side by side, and are folded behind them; the first one's row
-        has their number above the segment's); the bits are the same either way."""
-        tile, many = int(self.run.axk_kv4_prefill_tile()), int(self.run.axk_kv4_prefill_many())
+        cut there where a step has few tiles: its segments then run side by side, and are folded behind them.  Rows are of five numbers then,
+        the last of a cut tile's first row its segments, else 0.  The bits are the same either way."""
+        tile = int(self.run.axk_kv4_prefill_tile())
         segment_of, start_of = self.run.axk_kv4_prefill_segment, self.run.axk_kv4_prefill_segment_start
         runs = []
         for start, length, at in spans:
@@ -1872,20 +1872,21 @@ class Kernels:
         # two workgroups of one head fit a CU: fewer than that, and tiles are cut (a tile at 30,000 positions alone takes 28 of 256 CUs
         # 0.8 ms, and cut 0.2)
         cut = len(runs) * n_heads < 512
-        rows, slots = [], 0
+        rows, slots, any_cut = [], 0, 0
         for start, n, low, high in runs:
             first, last = int(segment_of(low)), int(segment_of(high))
             if first == last:
-                rows.append((high - low, start, n, -1, -1))
-            elif not cut or last - first >= 1 << 31 - many - 1:
-                rows.append((high - low, start, n, -1, slots))
+                rows.append((high - low, start, n, -1, -1, 0))
+            elif not cut:
+                rows.append((high - low, start, n, -1, slots, 0))
                 slots += 1
             else:
-                rows += [(min(high, int(start_of(s + 1)) - 1) - max(low, int(start_of(s))), start, n,
-                          s | (last - first + 1 << many if s == first else 0), slots + s - first) for s in range(first, last + 1)]
+                rows += [(min(high, int(start_of(s + 1)) - 1) - max(low, int(start_of(s))), start, n, s, slots + s - first,
+                          last - first + 1 if s == first else 0) for s in range(first, last + 1)]
                 slots += last - first + 1
+                any_cut = 1
         rows.sort(key=lambda r: -r[0])
-        return [r[1:] for r in rows]
+        return [r[1:5 + any_cut] for r in rows]
 
     def kv4_prefill_workspace(self, tiles, n_heads: int, head_dim: int) -> int:
         """Floats of `kv4_attention_prefill`'s workspace for these tiles (as `kv4_prefill_tiles` lists them)."""
@@ -1893,7 +1894,7 @@ class Kernels:
 
     def kv4_attention_prefill(self, q, q_stride, k_cache, v_cache, block_table, positions, seq_rows, out, tiles, partial, n_heads,
                               n_kv_heads, head_dim, page_size, window, scale) -> torch.Tensor:
-        """`attention_prefill` over a cache held in 4 bits: prompt portions by `kv4_prefill_tiles` (int32 [n, 4] on the device); partial:
+        """`attention_prefill` over a cache held in 4 bits: prompt portions by `kv4_prefill_tiles` (int32 [n, 4 or 5] on the device); partial:
         float32, `kv4_prefill_workspace` of these tiles.  Rows of no tile are left as they are."""
         what = "kv4_attention_prefill"
         T, stream = self._kv4_step(what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, q, out, tiles,
@@ -1901,11 +1902,14 @@ class Kernels:
         self._kv4_rows(what, q, q_stride, out, T, n_heads, head_dim)
         if partial.dtype is not _F32 or not partial.is_contiguous() or tiles.dtype is not _I32 or not tiles.is_contiguous():
             raise KernelError(f"{what}: a workspace of {partial.dtype}, tiles of {tiles.dtype}: expected contiguous float32 and int32")
-        if tiles.numel() and (tiles.dim() != 2 or tiles.shape[1] != 4):
+        n_tiles, columns = tiles.shape if tiles.dim() == 2 else (-1 if tiles.numel() else 0, 4)
+        if n_tiles < 0 or n_tiles > 0 and not 4 <= columns <= 5:
             raise KernelError(f"{what}: tiles {tuple(tiles.shape)}")
+        if n_tiles == 0:
+            return out
         rc = self.run.axk_kv4_attention_prefill(
             q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), block_table.shape[1], positions.data_ptr(),
-            seq_rows.data_ptr(), out.data_ptr(), tiles.data_ptr(), tiles.numel() // 4, partial.data_ptr(), partial.numel(), n_heads, n_kv_heads,
+            seq_rows.data_ptr(), out.data_ptr(), tiles.data_ptr(), n_tiles, columns, partial.data_ptr(), partial.numel(), n_heads, n_kv_heads,
             head_dim, page_size, window, float(scale), stream)
         if rc != 0:
             self._check(rc)

@@ -28,21 +28,21 @@ def test_tiles_have_every_row_and_position_once(seed, nh, nkv, window):
     tiles = k.kv4_prefill_tiles(spans, window, nh, nkv)
     start, segment = k.run.axk_kv4_prefill_segment_start, k.run.axk_kv4_prefill_segment
     at_of = {s + i: at + i for s, n, at in spans for i in range(n)}
-    rows, slots, parts, work, many = [], set(), {}, [], int(k.run.axk_kv4_prefill_many())
-    for first, count, which, slot in tiles:
+    rows, slots, parts, work = [], set(), {}, []
+    assert len({len(row) for row in tiles}) == 1 and (len(tiles[0]) == 5) == any(row[2] >= 0 for row in tiles)
+    for first, count, which, slot, *n in tiles:
         assert 0 < count <= TILE
         p0, p1 = at_of[first], at_of[first + count - 1]
         assert p1 - p0 == count - 1                       # one portion's
         low = max(0, p0 + 1 - window) if window else 0
         s0, s1 = segment(low), segment(p1)
         if which >= 0:
-            n, which = which >> many, which & ((1 << many) - 1)
-            assert s0 <= which <= s1 and slot not in slots and n == (s1 - s0 + 1 if which == s0 else 0)
+            assert s0 <= which <= s1 and slot not in slots and n == [s1 - s0 + 1 if which == s0 else 0]
             slots.add(slot)
             parts.setdefault((first, count), {})[which] = slot
             work.append(min(p1, start(which + 1) - 1) - max(low, start(which)))
         else:
-            assert which == -1 and (slot == -1) == (s0 == s1) and slot not in slots
+            assert which == -1 and n in ([], [0]) and (slot == -1) == (s0 == s1) and slot not in slots
             rows += range(first, first + count)
             slots |= {slot} - {-1}
             work.append(p1 - low)
@@ -61,9 +61,9 @@ def test_segments_follow_each_other():
     k = kernels("bfloat16")
     segment, start = k.run.axk_kv4_prefill_segment, k.run.axk_kv4_prefill_segment_start
     for s in range(300):
-        assert start(s) < start(s + 1) and start(s) % 64 == 0 and s < 1 << int(k.run.axk_kv4_prefill_many())
+        assert start(s) < start(s + 1) and start(s) % 64 == 0
         assert segment(start(s)) == s == segment(start(s + 1) - 1)
-    assert 0 < segment(2 ** 31 - 1) < 1 << int(k.run.axk_kv4_prefill_many()) and start(segment(2 ** 31 - 1) + 1) == 2 ** 31 - 1
+    assert segment(2 ** 31 - 1) > 0 and start(segment(2 ** 31 - 1) + 1) == 2 ** 31 - 1
 
 
 @pytest.mark.parametrize("window", [0, 1, 300, 9000])
@@ -98,7 +98,7 @@ def test_entry_points_refuse(dtype):
     read = dict(k=A, v=A, block_table=A, table_stride=1, pos=A, rows=A, k_out=A, v_out=A, n=1, nkv=2, hd=64, page=16, stream=None)
     decode = dict(q=A, q_stride=256, k=A, v=A, block_table=A, table_stride=1, pos=A, rows=A, out=A, index=None, T=1, work=A, n_work=1,
                   partial=A, chunks=1, nh=4, nkv=2, hd=64, page=16, window=0, scale=0.1, stream=None)
-    prompt = dict(q=A, q_stride=256, k=A, v=A, block_table=A, table_stride=1, pos=A, rows=A, out=A, tiles=A, n=1, partial=A, floats=4, nh=4,
+    prompt = dict(q=A, q_stride=256, k=A, v=A, block_table=A, table_stride=1, pos=A, rows=A, out=A, tiles=A, n=1, columns=4, partial=A, floats=4, nh=4,
                   nkv=2, hd=64, page=16, window=0, scale=0.1, stream=None)
     cases = [(run.axk_rope_kv4_write, write, [dict(T=-1), dict(nh=0), dict(nkv=0), dict(hd=96), dict(hd=32), dict(page=4), dict(page=2048),
                                               dict(page=24), dict(rot=8), dict(rot=80), dict(rot=-16), dict(qkv=A + 8), dict(q_out=A + 4),
@@ -110,7 +110,7 @@ def test_entry_points_refuse(dtype):
                                                      dict(chunks=1025), dict(n_work=-1), dict(work=None), dict(partial=None), dict(partial=A + 4),
                                                      dict(q=A + 8), dict(out=A + 8), dict(q_stride=257), dict(q_stride=-256)]),
              (run.axk_kv4_attention_prefill, prompt, [dict(hd=80), dict(page=12), dict(nh=5), dict(nh=65536), dict(window=-1), dict(scale=-1.0),
-                                                      dict(n=-1), dict(n=65536), dict(tiles=None), dict(floats=-1), dict(partial=None),
+                                                      dict(n=-1), dict(n=65536), dict(tiles=None), dict(columns=3), dict(columns=6), dict(floats=-1), dict(partial=None),
                                                       dict(partial=A + 4), dict(k=A + 8), dict(q_stride=257)])]
     for entry, good, wrong in cases:
         for change in wrong:

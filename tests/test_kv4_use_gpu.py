@@ -99,7 +99,7 @@ def test_captured_and_replayed(dtype):
     partial = torch.zeros(k.kv4_decode_workspace(3, nh, dim, chunks), device="cuda")
     lists = [k.kv4_prefill_tiles([(3, n, p[3])], 0, nh, nkv) for p in pos_host]
     rows = max(len(t) for t in lists)
-    lists = [t + [(0, 0, -1, -1)] * (rows - len(t)) for t in lists]
+    lists = [t + [(0, 0, -1, -1, 0)] * (rows - len(t)) for t in lists]
     tiles = i32(lists[0])
     state = torch.zeros(max(k.kv4_prefill_workspace(t, nh, dim) for t in lists), device="cuda")
     out = torch.zeros((T, nh * dim), dtype=qkv.dtype, device="cuda")
@@ -275,7 +275,7 @@ def test_one_and_two_heads_a_workgroup_give_the_same_bits(dim, nh, nkv, spans, w
     assert max(few) <= 768
     nothing = [(0, 0, -1, -1)] * (769 // nh + 1)
     want = None
-    for tiles in (cut, cut + nothing, whole, nothing + whole):
+    for tiles in (cut, cut + [row + (0,) * (len(cut[0]) - 4) for row in nothing], whole, nothing + whole):
         out = torch.full((T, nh * dim), 5.0, dtype=q.dtype, device="cuda")
         partial = torch.full((k.kv4_prefill_workspace(tiles, nh, dim),), float("nan"), device="cuda")
         k.kv4_attention_prefill(q, nh * dim, *held.args, i32(pos), i32(seq), out, i32(tiles), partial, nh, nkv, dim, page, window, 0.1)
