@@ -170,8 +170,9 @@ KV4_SINGLES = 16        # portions of up to so many tokens go token by token to 
 
 
 class Kv4Plan:
-    """How the 4-bit cache's kernels split a step: portions of more than 16 tokens by tiles, the others token by token (16 tokens at
-    4,000 positions 17 us so, 60 by a tile; by its length alone, so that a portion's bits do not depend on the step).  Made once per
+    """How the 4-bit cache's kernels split a step: portions of more than 16 tokens by tiles, the others token by token, by the portion's
+    length alone, so that its bits do not depend on the step.  (Of 28 query and 4 key/value heads: 16 tokens at 4,000 positions 17 us so, 60
+    by a tile; 32 at 2,000 alone 18 and 50, but eight such portions 100 and 50, and with 32 key/value heads 68 and 49.)  Made once per
     step and window, shared by all layers."""
 
     def __init__(self, ctx, window: int, n_heads: int, n_kv_heads: int, head_dim: int):
