@@ -284,3 +284,31 @@ def test_one_and_two_heads_a_workgroup_give_the_same_bits(dim, nh, nkv, spans, w
     assert want.isnan().any() and want.isfinite().any() and not (want == 5.0).all(-1).any()
     single = decode(k, held, q, pos, seq, nh, nkv, dim, page, window, 0.1)
     assert torch.equal(single.isnan(), want.isnan())
+
+
+def test_places_beyond_32_bits():
+    """Pages that begin beyond 4 GiB of a cache: written, read back and attended to as the same positions in the first pages are."""
+    k, nh, nkv, dim, page = kernels("bfloat16"), 8, 8, 128, 1024
+    n_pages = (9 << 29) // (nkv * page * P.row_bytes(dim)) + 3
+    assert (n_pages - 2) * nkv * page * P.row_bytes(dim) > 1 << 32
+    caches = [torch.empty((n_pages, nkv, page, P.row_bytes(dim)), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    for c in caches:
+        c[:2] = c[-2:] = 255                                         # (nothing else is looked at)
+    n = 1100
+    x = torch.from_numpy(random_rows(np.random.default_rng(1), n, nh + 2 * nkv, dim).reshape(n, -1)).bfloat16().cuda()
+    angles = torch.randn((n, 32, 2), generator=torch.Generator().manual_seed(2)).cuda()
+    pos, seq = list(range(n)), [0] * n
+    got = []
+    for table in (i32([[1, 0]]), i32([[n_pages - 1, n_pages - 2]])):
+        q = torch.empty((n, nh * dim), dtype=x.dtype, device="cuda")
+        k.rope_kv4_write(x, q, angles, i32(pos), i32(seq), table, *caches, nh, nkv, dim, 64, page)
+
+        class Held:
+            args = (*caches, table)
+        back = [torch.empty((n, nkv, dim), dtype=x.dtype, device="cuda") for _ in range(2)]
+        k.kv4_read(*caches, table, i32(pos), i32(seq), *back, nkv, dim, page)
+        some = [1, 700, 1023, 1024, 1099]
+        got.append([q, *back, prefill(k, Held, q, [(n, 0)], [0], nh, nkv, dim, page, 0, 0.05)[2],
+                    decode(k, Held, q[some].contiguous(), some, [0] * 5, nh, nkv, dim, page, 0, 0.05)])
+    for low, high in zip(*got):
+        assert torch.equal(low.view(torch.int16), high.view(torch.int16)) and low.isfinite().all()
