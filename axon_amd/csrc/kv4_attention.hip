@@ -45,11 +45,17 @@ __device__ __forceinline__ void kv4_split(const float (&x)[8], u32x4 (&out)[TERM
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const half2_t h = {(_Float16)rest[2 * i], (_Float16)rest[2 * i + 1]};
-      out[n][i] = __builtin_bit_cast(unsigned, h);
+      unsigned pair = __builtin_bit_cast(unsigned, h);
       if (n + 1 < TERMS) {
-        rest[2 * i] = __fsub_rn(rest[2 * i], (float)h[0]);
-        rest[2 * i + 1] = __fsub_rn(rest[2 * i + 1], (float)h[1]);
+        // what is left of each, exactly, out of the pair in one instruction (from h the compiler rounds each number once more alone: 256 for
+        // 32 numbers in place of 112; 1,000 tokens of 14 heads of 64 dims in a window of 700 42 -> 38 us)
+        float left;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(left) : "v"(pair), "v"(rest[2 * i]));
+        rest[2 * i] = left;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(left) : "v"(pair), "v"(rest[2 * i + 1]));
+        rest[2 * i + 1] = left;
       }
+      out[n][i] = pair;
     }
   }
 }
