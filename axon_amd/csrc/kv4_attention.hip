@@ -899,6 +899,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
           w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], c, add));
           sum[i & 1] = __fadd_rn(sum[i & 1], w[i]);
         }
+        asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));       // (added here, beside products: else behind the last of them, 1 to 2 % later)
         kv4_split(w, pf);
         if (st + 1 < 4) wait_lgkmcnt<DT>();
         else wait_lgkmcnt<0>();
