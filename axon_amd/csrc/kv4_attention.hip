@@ -24,6 +24,7 @@
 #define KV4_COLUMNS 16             // query heads of a key head that a wave takes at a time
 #define KV4_RAISE 8.0f             // how far (log2) scores may pass the reference before it is raised
 #define KV4_WEIGHT 7.0f            // log2 of a weight at the reference: at most 2^15 goes to half precision
+#define KV4_FAR 4096.0f            // references (log2) beyond which scores have theirs taken off before their factor (kv4_offset)
 #define LOG2E 1.4426950408889634f
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -75,14 +76,26 @@ __host__ __device__ inline int kv4_chunk(int seen) {
   return rounds * KV4_WAVES * KV4_BLOCK;
 }
 
-// The weights are taken relative to a reference, which is raised to a block's maximum only where that is KV4_RAISE or more above it
-// (the first block's always): what was summed before is then scaled by the factor returned, 1 for a column whose
-// reference stays.  A column's arithmetic depends on its own scores alone.
-__device__ __forceinline__ float kv4_raise(float& ref, float block_max) {
-  const bool up = block_max > ref + KV4_RAISE;
+// The weights are taken relative to a reference, a score as the products leave it (times c: its log2), which is raised to a block's maximum
+// only where that is KV4_RAISE or more above it (the first block's always): what was summed before is then scaled by the factor
+// returned, 1 for a column whose reference stays.  A column's arithmetic depends on its own scores alone.
+__device__ __forceinline__ float kv4_raise(float& ref, float block_max, float c) {
+  const bool up = __fmul_rn(__fsub_rn(block_max, ref), c) > KV4_RAISE;        // (nothing seen yet, and nothing now: not a number, so no)
   const float before = ref;
   ref = up ? block_max : ref;
-  return up ? __builtin_amdgcn_exp2f(__fsub_rn(before, ref)) : 1.0f;
+  return up ? __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(before, ref), c)) : 1.0f;
+}
+
+// What a score s c has added to it for its weight's log2.  ref c rounded and KV4_WEIGHT less that rounded are off by 2^-13 each up to KV4_FAR,
+// for all of a reference's weights alike.  At 2^25 they would be off by more than KV4_WEIGHT, and weights out of half precision's range:
+// a column beyond KV4_FAR has its reference taken off its scores instead (subtract(reference), which is 0 for the wave's other
+// columns and leaves them as they are), exactly where it matters, near the largest.
+template <typename Subtract>
+__device__ __forceinline__ float kv4_offset(float ref, float c, Subtract subtract) {
+  const float at = __fmul_rn(ref, c);
+  const bool far = fabsf(at) > KV4_FAR && fabsf(ref) < INFINITY;
+  if (__any(far)) subtract(far ? ref : 0.0f);
+  return ref == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, far ? 0.0f : at);
 }
 
 // ============================================================================ single tokens
@@ -208,12 +221,17 @@ __device__ __forceinline__ void kv4_weights(f32x4 (&s)[4], bool whole, int p0, i
     for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
   mx = fmaxf(mx, __shfl_xor(mx, 16, AXON_WAVE));
   mx = fmaxf(mx, __shfl_xor(mx, 32, AXON_WAVE));
-  const float factor = kv4_raise(ref, __fmul_rn(mx, c));
+  const float factor = kv4_raise(ref, mx, c);
   if (__any(factor != 1.0f)) {
     l = __fmul_rn(l, factor);
     rescale(factor);
   }
-  const float add = ref == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, ref);
+  const float add = kv4_offset(ref, c, [&](float off) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[t][r] = __fsub_rn(s[t][r], off);
+  });
   float sum = 0.0f;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -380,6 +398,7 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
     }
     l = __fadd_rn(l, __shfl_xor(l, 16, AXON_WAVE));
     l = __fadd_rn(l, __shfl_xor(l, 32, AXON_WAVE));
+    ref = __fmul_rn(ref, c);                   // (what is joined is compared as log2)
   }
   if (l16 < columns) {
 #pragma unroll
@@ -600,7 +619,8 @@ __device__ __forceinline__ void kv4_meet() {       // everyone's part of the sta
   asm volatile("" ::: "memory");
 }
 
-// A wave's state of a segment: its rows' outputs, references and (each half of the wave its own) sums.  Kept as the lanes hold it.
+// A wave's state of a segment: its rows' outputs, references (in the workspace their log2) and (each half of the wave its own) sums.  Kept as the
+// lanes hold it.
 template <int HD>
 struct Kv4State {
   f32x16 o[HD / 32];
@@ -871,7 +891,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
         for (int e = 0; e < 16; ++e) mx[pt] = fmaxf(mx[pt], s[pt][e]);
       float top = fmaxf(mx[0], mx[1]);
       top = fmaxf(top, __shfl_xor(top, 32, AXON_WAVE));
-      const float factor = kv4_raise(ref, __fmul_rn(top, c));
+      const float factor = kv4_raise(ref, top, c);
       if (__any(factor != 1.0f)) {
         l = __fmul_rn(l, factor);
 #pragma unroll
@@ -879,7 +899,12 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[dt][e] = __fmul_rn(o[dt][e], factor);
       }
-      const float add = ref == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, ref);
+      const float add = kv4_offset(ref, c, [&](float off) {
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[pt][e] = __fsub_rn(s[pt][e], off);
+      });
       // The weights of sixteen positions, then their products with all dims: on those the matrix cores work while the vector unit has the
       // weights of the next sixteen.
       float sum[2] = {0.0f, 0.0f};
@@ -922,6 +947,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   }
   for (; b < seg_end; ++b) pass(b);
   if (!live || (segment < 0 && seg_first == seg_last)) continue;
+  ref = __fmul_rn(ref, c);                         // (what is folded is compared as log2)
   if (kept) kv4_fold<HD, true>(st, state_at, wave & 3, lane, 0);
   if (seg_end < n_blocks || segment >= 0) {
     kv4_store<HD>(st, state_at, wave & 3, lane, nan_groups);
