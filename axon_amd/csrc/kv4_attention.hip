@@ -66,6 +66,10 @@ __device__ __forceinline__ int kv4_query_shift(float largest) {
   return largest > 0.0f && largest < INFINITY ? 14 - ilogbf(largest) : 0;
 }
 
+// A score's factor to log2, which takes the query's power of two back.  Of the smallest queries it is below all numbers, and would be 0, which is
+// not a number with what a masked place holds: 2^-126 in its place leaves scores (up to 2^38 before it) that are nothing to 32 bits either.
+__device__ __forceinline__ float kv4_score_factor(float scale, int shift) { return fmaxf(ldexpf(scale * LOG2E, -shift), 0x1p-126f); }
+
 // Positions of a chunk of a token that sees `seen` positions: by the token alone, so that its result does not depend on what else a
 // step holds.  Up to 8,192 positions every wave has one block, which spreads a token over the chip; a longer one pays for
 // its partial results.  28 heads over 4 of 128, us, attention + join, one block a wave / up to four: 1 token at 8,192 5.9 + 3.4 / 11.4 + 3.0, at
@@ -318,7 +322,7 @@ __device__ __forceinline__ float kv4_operands(Kv4Queries<HD>& q, float scale, u3
     for (int i = 0; i < 8; ++i) q.x[j][i] = q.x[j][i] * up * up2;
     kv4_split(q.x[j], qf[j]);
   }
-  return ldexpf(scale * LOG2E, -shift);
+  return kv4_score_factor(scale, shift);
 }
 
 // A workgroup has a chunk of a token and a set of up to sixteen query heads of a key head: grid (key heads x sets, work items).  Each of its
@@ -784,7 +788,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
       for (int i = 0; i < 8; ++i) x[ks][i] = x[ks][i] * up * up2;
       kv4_split(x[ks], qf[ks]);
     }
-    c = ldexpf(scale * LOG2E, -by);
+    c = kv4_score_factor(scale, by);
   }
   Kv4State<HD> st;
   f32x16(&o)[DT] = st.o;

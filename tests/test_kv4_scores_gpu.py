@@ -1,4 +1,4 @@
-"""Attention over the 4-bit cache where scores are very large: both kernels, one chunk and several, one segment and
+"""Attention over the 4-bit cache where scores are very large or nothing at all: both kernels, one chunk and several, one segment and
 several.
 
 Behind a gap of 64 or more (natural logarithms, beyond twice what 32 bits can lose of a score: test_kv4_gpu.py's (dim + 8) 2^-24 of
@@ -66,3 +66,19 @@ def test_scores_of_any_size(dtype, dim, at, window, same):
     # the first position alone, whose score is of either sign: its value
     early = decode(k, held, q, [0] * n, seq, nh, nkv, dim, page, window, 0.09)
     assert check_sharp(dtype, early, q, held, [0] * n, window, 0.09, dim, nh) == n * nh
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.09, 2.0 ** -100])
+@pytest.mark.parametrize("dim,at,window", [(128, 70, 0), (64, 1100, 90)])
+def test_queries_next_to_nothing(dtype, scale, dim, at, window):
+    """Rows of the smallest numbers there are: every position seen has the same weight, and none that is not."""
+    nh, nkv, page, n = 4, 2, 16, 12
+    k, held = kernels(dtype), Held([at + n], nkv, dim, page, seed=91)
+    smallest = torch.finfo(TORCH[dtype]).smallest_normal * torch.finfo(TORCH[dtype]).eps
+    sign = torch.randn((n, nh * dim), generator=torch.Generator().manual_seed(8)).sign().double()
+    q = (sign * smallest * torch.exp2(torch.arange(n).double() * 3)[:, None]).to(TORCH[dtype]).cuda()
+    assert (q != 0).all()
+    pos, seq, rows = prefill(k, held, q, [(n, at)], [0], nh, nkv, dim, page, window, scale)
+    check(dtype, rows, q, held, pos, seq, window, scale, dim, nh)
+    check(dtype, decode(k, held, q, pos, seq, nh, nkv, dim, page, window, scale), q, held, pos, seq, window, scale, dim, nh)
