@@ -231,7 +231,8 @@ class LLM:
                     logits = self.engine.run_prepared([reqs[p.id].tokens[p.start] for p in plan])
                 else:
                     entries = [StepEntry(p.id, reqs[p.id].tokens[p.start:p.start + p.count],
-                                         [p.count - 1] if p.wants_logits else []) for p in plan]
+                                         [p.count - 1] if p.wants_logits else [],
+                                         max(0, min(p.count, reqs[p.id].prompt_len - p.start))) for p in plan]
                     logits = self.engine.step(entries)
                 stats.steps += 1
                 wanted = [p for p in plan if p.wants_logits]
@@ -316,7 +317,7 @@ class LLM:
         rid = ("logits", self._next_id)
         self._next_id += 1
         want = list(range(len(ids))) if all_positions else [len(ids) - 1]
-        out = self.engine.step([StepEntry(rid, ids, want)], end=[rid]).clone()     # a one-token step returns a view
+        out = self.engine.step([StepEntry(rid, ids, want, len(ids))], end=[rid]).clone()     # a one-token step returns a view
         return out if all_positions else out[0]
 
 

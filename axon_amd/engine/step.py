@@ -36,19 +36,30 @@ class StepError(ValueError):
 
 @dataclass
 class StepEntry:
+    """`prompt`: how many of the tokens, from the first on, are the request's prompt's (the others it generated).  Only a model with
+    `Mixer.prompt_apart` asks; None: all of two or more tokens, none of a single one."""
     id: Hashable
     tokens: Sequence[int]
     want: Sequence[int] = ()
+    prompt: Optional[int] = None
 
 
 @dataclass
 class Span:
-    """One entry as the parts see it: its slot, where its tokens lie in the batch, and the
-    position of its first token."""
+    """One entry as the parts see it: its slot, where its tokens lie in the batch, the
+    position of its first token, and what it says of its prompt."""
     slot: int
     q_start: int
     q_len: int
     start_pos: int
+    prompt: Optional[int] = None
+
+    @property
+    def prompt_tokens(self) -> int:
+        """How many of its tokens, from the first on, are the prompt's (see StepEntry)."""
+        if self.prompt is None:
+            return self.q_len if self.q_len > 1 else 0
+        return self.prompt
 
 
 @dataclass
@@ -115,6 +126,7 @@ class Engine:
                 raise StepError(f"max_seq_len {self.max_seq_len}: a mixer of this model takes contexts of up to {limit}")
             if not b.mixer.takes_page_size(cfg.page_size):
                 raise StepError(f"page_size {cfg.page_size}: a mixer of this model takes other cache pages (its kernels: powers of two from 8 to 1024)")
+        self._prompt_apart = any(b.mixer.prompt_apart for b in model.blocks)
         # workspaces mixers want in decoding steps (Mixer.decode_scratch): one per name, sized for the
         # most requests and the longest context, allocated at the first decoding step (the pool leaves room for them)
         self._scratch_sizes: Dict = {}
@@ -265,6 +277,9 @@ class Engine:
                     self.live[e.id] = LiveRequest(self.cache.open())
                     opened.append(e.id)
             meta, want_rows, counts = self._layout(entries)
+            for e, n in zip(entries, counts):
+                if e.prompt is not None and not (hasattr(e.prompt, "__index__") and 0 <= int(e.prompt) <= n):
+                    raise StepError(f"request {e.id!r}: {e.prompt!r} of its {n} tokens as the prompt's")
             self.cache.reserve_many([(self.live[e.id].slot, self.live[e.id].n_cached + int(n)) for e, n in zip(entries, counts)])
         except Exception:
             for rid in opened:
@@ -280,11 +295,12 @@ class Engine:
             spans, at = [], 0
             for e, n in zip(entries, counts):
                 req = self.live[e.id]
-                spans.append(Span(req.slot, at, int(n), req.n_cached))
+                spans.append(Span(req.slot, at, int(n), req.n_cached, None if e.prompt is None else int(e.prompt)))
                 at += int(n)
             T = at
             self.cache.sync_tables()
-            if T == len(entries) and len(want_rows) == T and T <= self.cfg.max_seqs:
+            apart = self._prompt_apart and any(s.prompt_tokens for s in spans)        # (a prompt's single token is not decoded)
+            if T == len(entries) and len(want_rows) == T and T <= self.cfg.max_seqs and not apart:
                 logits = self._decode_step(meta[0].tolist(), meta[1].tolist(), meta[2].tolist(), spans)
                 self._last_decode = [e.id for e in entries]
             else:

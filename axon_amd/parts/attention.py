@@ -13,10 +13,10 @@ Parameters: `hidden_size`, `num_heads`, `num_kv_heads`, `head_dim`, `qkv_bias` (
 or "optional"), `out_bias`, `window` (0: all earlier positions), `position` (a PartSpec).
 
 `hold_cache_in(4)`: keys and values in 4 bits with a scale and a zero for 32 dims (head sizes 64 and 128).  The
-projection is then a plain product, the rotation quantises what it stores, and portions of up to 16 tokens go token by token.
-A token's bits do not depend on what else is in a step, and a portion's not on how it is cut into larger ones; but the kernel for
-single tokens and the one for portions sum in orders of their own, so a position that came as a single token (or was decoded) and the same one in
-a portion of more agree within their rounding, not bit for bit.
+projection is then a plain product, and the rotation quantises what it stores.  The kernel for prompt portions and the one for single tokens
+sum in orders of their own: a prompt's tokens go to the first, however they are cut, and those that a request generated to the second,
+also where a request that gave way is fed again.  So a token's bits do not depend on what else is in a step, nor on how its request was
+cut; but a token that is a prompt's and the same one generated agree within their rounding, not bit for bit.
 """
 from __future__ import annotations
 
@@ -166,38 +166,38 @@ def decode_scratch_floats(k, window: int, n_heads: int, head_dim: int, max_seqs:
 
 
 NORMED_ROWS = 16        # the most rows that a product takes with the norm of its operand inside (`gemm_normed_ok`)
-KV4_SINGLES = 16        # portions of up to so many tokens go token by token to the 4-bit cache's kernel for single tokens
+KV4_PARTIAL = 1 << 25   # floats of partial results (128 MiB) that a call for single tokens of the 4-bit cache may want; more tokens are more calls
 
 
 class Kv4Plan:
-    """How the 4-bit cache's kernels split a step: portions of more than 16 tokens by tiles, the others token by token, by the portion's
-    length alone, so that its bits do not depend on the step.  (Of 28 query and 4 key/value heads: 16 tokens at 4,000 positions 17 us so, 60
-    by a tile; 32 at 2,000 alone 18 and 50, but eight such portions 100 and 50, and with 32 key/value heads 68 and 49.)  Made once per
-    step and window, shared by all layers."""
+    """How the 4-bit cache's kernels split a step: tokens of prompts by tiles, whatever a portion's length, and tokens that requests generated
+    one by one (of a request that gave way and is fed again many, in calls whose workspace stays small), so that a token's bits do not
+    depend on the step.  (Few tokens far into a request would be quicker one by one: of 28 query and 4 key/value heads 16 tokens at
+    4,000 positions 17 us, by a tile 60.)  Made once per step and window, shared by all layers."""
 
     def __init__(self, ctx, window: int, n_heads: int, n_kv_heads: int, head_dim: int):
         k, dev = ctx.rt.k, ctx.rt.device
-        self.tiles = self.tile_partial = self.decode_tokens = None
+        self.tiles = self.tile_partial = self.partial = None
+        self.singles = []                    # (tokens, their work list, most chunks) a call
         if ctx.decode_only:
-            self.decode_tokens = ctx.n_tokens
-            self.max_chunks = ctx.decode_shapes[("kv4_chunks", window)]
-            self.decode_work = ctx.decode_inputs[("kv4_work", window)]
+            self.singles.append((ctx.n_tokens, ctx.decode_inputs[("kv4_work", window)], ctx.decode_shapes[("kv4_chunks", window)]))
             self.partial = ctx.decode_scratch[("kv4_partial", window, n_heads, head_dim)]
             return
         if any(s.q_len < 1 or s.q_start < 0 or s.q_start + s.q_len > ctx.n_tokens for s in ctx.spans):
             raise ValueError("attention plan: a span lies outside the tokens of the step")
-        short = [s for s in ctx.spans if s.q_len <= KV4_SINGLES]
-        portions = [(s.q_start, s.q_len, s.start_pos) for s in ctx.spans if s.q_len > KV4_SINGLES]
+        portions = [(s.q_start, s.prompt_tokens, s.start_pos) for s in ctx.spans if s.prompt_tokens > 0]
+        tokens = [s.q_start + i for s in ctx.spans for i in range(s.prompt_tokens, s.q_len)]
+        at = [s.start_pos + i for s in ctx.spans for i in range(s.prompt_tokens, s.q_len)]
         if portions:
             rows = k.kv4_prefill_tiles(portions, window, n_heads, n_kv_heads)
             self.tiles = upload(rows, dev)
             self.tile_partial = torch.empty(k.kv4_prefill_workspace(rows, n_heads, head_dim), dtype=torch.float32, device=dev)
-        if short:
-            at = [s.start_pos + i for s in short for i in range(s.q_len)]
-            self.decode_tokens = upload([s.q_start + i for s in short for i in range(s.q_len)], dev)
-            self.max_chunks = k.kv4_decode_chunks(at, window)
-            self.decode_work = upload(k.kv4_decode_work(at, window), dev)
-            self.partial = torch.empty(k.kv4_decode_workspace(len(at), n_heads, head_dim, self.max_chunks), dtype=torch.float32, device=dev)
+        if tokens:
+            chunks = k.kv4_decode_chunks(at, window)
+            most = min(len(at), max(1, KV4_PARTIAL // k.kv4_decode_workspace(1, n_heads, head_dim, chunks)))
+            self.partial = torch.empty(k.kv4_decode_workspace(most, n_heads, head_dim, chunks), dtype=torch.float32, device=dev)
+            for i in range(0, len(at), most):
+                self.singles.append((upload(tokens[i:i + most], dev), upload(k.kv4_decode_work(at[i:i + most], window), dev), chunks))
 
 
 class GQAttention(Mixer):
@@ -251,6 +251,7 @@ class GQAttention(Mixer):
         if self.position is not None and self.position.rotary_dim % 16:
             raise ConfigError(f"a cache in {bits} bits rotates a multiple of 16 dims, not {self.position.rotary_dim}")
         self.cache_bits = bits
+        self.prompt_apart = True
 
     def takes_page_size(self, page_size: int) -> bool:
         return self.cache_bits == 0 or self._kernels is None or self._kernels.kv4_ok(self.hd, page_size)
@@ -418,9 +419,8 @@ class GQAttention(Mixer):
         common = (q, qkv.stride(0), k_cache, v_cache, group.block_table, ctx.positions, ctx.seq_rows, att)
         if plan.tiles is not None:
             k.kv4_attention_prefill(*common, plan.tiles, plan.tile_partial, *sizes, group.page_size, self.window, self.scale)
-        if plan.decode_tokens is not None:
-            k.kv4_attention_decode(*common, plan.decode_tokens, plan.partial, plan.max_chunks, *sizes, group.page_size, self.window,
-                                   self.scale, work=plan.decode_work)
+        for tokens, work, chunks in plan.singles:
+            k.kv4_attention_decode(*common, tokens, plan.partial, chunks, *sizes, group.page_size, self.window, self.scale, work=work)
         k.gemm(att, self.w_o, residual, self.b_o, MODE_ADD_F32,
                following_norm=None if following is None else following.as_argument())
 

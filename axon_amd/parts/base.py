@@ -168,6 +168,10 @@ class PositionEncoding(Part):
 
 
 class Mixer(Part):
+    # Whether tokens of a request's prompt and tokens that it generated go to kernels whose sums are ordered differently: the step then tells
+    # them apart by their spans (`Span.prompt_tokens`), never by how they came, so that a request's bits do not depend on other requests.
+    prompt_apart = False
+
     def cache_spec(self) -> Optional[CacheSpec]:
         return None
 
