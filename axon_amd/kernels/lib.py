@@ -1888,20 +1888,29 @@ class Kernels:
         rows.sort(key=lambda r: -r[0])
         return [r[1:5 + any_cut] for r in rows]
 
+    @staticmethod
+    def kv4_prefill_slots(tiles) -> int:
+        """Slots of the workspace that these tiles (as `kv4_prefill_tiles` lists them) name."""
+        return max((row[3] + 1 for row in tiles), default=0)
+
     def kv4_prefill_workspace(self, tiles, n_heads: int, head_dim: int) -> int:
         """Floats of `kv4_attention_prefill`'s workspace for these tiles (as `kv4_prefill_tiles` lists them)."""
-        return int(self.run.axk_kv4_prefill_workspace(max((row[3] + 1 for row in tiles), default=0), n_heads, head_dim))
+        return int(self.run.axk_kv4_prefill_workspace(self.kv4_prefill_slots(tiles), n_heads, head_dim))
 
     def kv4_attention_prefill(self, q, q_stride, k_cache, v_cache, block_table, positions, seq_rows, out, tiles, partial, n_heads,
-                              n_kv_heads, head_dim, page_size, window, scale) -> torch.Tensor:
+                              n_kv_heads, head_dim, page_size, window, scale, slots: Optional[int] = None) -> torch.Tensor:
         """`attention_prefill` over a cache held in 4 bits: prompt portions by `kv4_prefill_tiles` (int32 [n, 4 or 5] on the device); partial:
-        float32, `kv4_prefill_workspace` of these tiles.  Rows of no tile are left as they are."""
+        float32, `kv4_prefill_workspace` of these tiles.  The tiles lie on the device, so how many slots they name is the caller's to say:
+        with `slots` (`kv4_prefill_slots` of them) a workspace that is too small is an error.  Without it the rows of tiles whose slot is
+        not there are left as they are, as rows of no tile are."""
         what = "kv4_attention_prefill"
         T, stream = self._kv4_step(what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, q, out, tiles,
                                    partial)
         self._kv4_rows(what, q, q_stride, out, T, n_heads, head_dim)
         if partial.dtype is not _F32 or not partial.is_contiguous() or tiles.dtype is not _I32 or not tiles.is_contiguous():
             raise KernelError(f"{what}: a workspace of {partial.dtype}, tiles of {tiles.dtype}: expected contiguous float32 and int32")
+        if slots is not None and (slots < 0 or partial.numel() < self.run.axk_kv4_prefill_workspace(slots, n_heads, head_dim)):
+            raise KernelError(f"{what}: workspace of {partial.numel()} floats is too small for {slots} slots")
         n_tiles, columns = tiles.shape if tiles.dim() == 2 else (-1 if tiles.numel() else 0, 4)
         if n_tiles < 0 or n_tiles > 0 and not 4 <= columns <= 5:
             raise KernelError(f"{what}: tiles {tuple(tiles.shape)}")

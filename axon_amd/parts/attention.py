@@ -190,7 +190,7 @@ class Kv4Plan:
         at = [s.start_pos + i for s in ctx.spans for i in range(s.prompt_tokens, s.q_len)]
         if portions:
             rows = k.kv4_prefill_tiles(portions, window, n_heads, n_kv_heads)
-            self.tiles = upload(rows, dev)
+            self.tiles, self.slots = upload(rows, dev), k.kv4_prefill_slots(rows)
             self.tile_partial = torch.empty(k.kv4_prefill_workspace(rows, n_heads, head_dim), dtype=torch.float32, device=dev)
         if tokens:
             chunks = k.kv4_decode_chunks(at, window)
@@ -418,7 +418,8 @@ class GQAttention(Mixer):
         plan = ctx.shared[key]
         common = (q, qkv.stride(0), k_cache, v_cache, group.block_table, ctx.positions, ctx.seq_rows, att)
         if plan.tiles is not None:
-            k.kv4_attention_prefill(*common, plan.tiles, plan.tile_partial, *sizes, group.page_size, self.window, self.scale)
+            k.kv4_attention_prefill(*common, plan.tiles, plan.tile_partial, *sizes, group.page_size, self.window, self.scale,
+                                    slots=plan.slots)
         for tokens, work, chunks in plan.singles:
             k.kv4_attention_decode(*common, tokens, plan.partial, chunks, *sizes, group.page_size, self.window, self.scale, work=work)
         k.gemm(att, self.w_o, residual, self.b_o, MODE_ADD_F32,
