@@ -1839,6 +1839,8 @@ class Kernels:
             n, index = token_index, None
         else:
             self._i32(token_index, "token_index")
+            if token_index.get_device() != positions.get_device():
+                raise KernelError(f"{what}: token_index on {token_index.device}, the step on {positions.device}")
             n, index = token_index.numel(), token_index.data_ptr()
         if partial.dtype is not _F32 or not partial.is_contiguous() or work.dtype is not _I32 or not work.is_contiguous() or work.dim() != 1:
             raise KernelError(f"{what}: a workspace of {partial.dtype}, a work list {tuple(work.shape)} of {work.dtype}: expected contiguous float32 "

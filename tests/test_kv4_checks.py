@@ -43,7 +43,8 @@ def calls(monkeypatch):
     k, noted = copy.copy(kernels("bfloat16")), []
     real = k.run
     own = {name: getattr(real, name) for name in ("axk_kv4_ok", "axk_kv4_row_bytes", "axk_kv4_decode_workspace", "axk_kv4_prefill_workspace",
-                                                  "axk_kv4_prefill_tile", "axk_kv4_prefill_segment", "axk_kv4_prefill_segment_start")}
+                                                  "axk_kv4_prefill_tile", "axk_kv4_prefill_segment", "axk_kv4_prefill_segment_start",
+                                                  "axk_kv4_decode_chunk", "axk_kv4_decode_item_factor")}
     for name in ("axk_kv4_attention_decode", "axk_kv4_attention_prefill"):
         own[name] = lambda *a, name=name: noted.append(name) or 0
     k.run = SimpleNamespace(**own)
@@ -71,3 +72,13 @@ def test_prompt_workspaces_that_are_too_small(calls):
     one = k.kv4_prefill_tiles([(0, 100, 0)], 0, NH, NKV)
     assert k.kv4_prefill_slots(one) == k.kv4_prefill_slots([]) == 0
     k.kv4_attention_prefill(**dict(arguments(100), tiles=i32(one), partial=on(torch.zeros(0)), slots=0))
+
+
+def test_named_tokens_on_another_device(calls):
+    k, noted = calls
+    good = dict(arguments(3), token_index=i32([2, 0]), partial=on(torch.zeros(k.kv4_decode_workspace(2, NH, DIM, 1))), max_chunks=1,
+                work=i32(k.kv4_decode_work([5, 5], 0)))
+    k.kv4_attention_decode(**good)
+    with pytest.raises(KernelError):
+        k.kv4_attention_decode(**{**good, "token_index": i32([2, 0], device=1)})
+    assert noted == ["axk_kv4_attention_decode"]
