@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes
 from collections import ChainMap
 from dataclasses import dataclass
+from functools import partial
 from typing import Dict, Hashable, Iterable, List, Optional, Sequence
 
 import numpy as np
@@ -135,8 +136,13 @@ class Engine:
             if asked is not None:
                 self._scratch_sizes[asked[0]] = max(self._scratch_sizes.get(asked[0], 0), int(asked[1]))
         self._scratch: Optional[Dict] = None
+        of_steps: Dict = {}                  # what mixers take for a step of prompts (Mixer.step_scratch)
+        for b in model.blocks:
+            asked = b.mixer.step_scratch(cfg.max_batch_tokens, cfg.max_seqs, self.max_seq_len)
+            if asked is not None:
+                of_steps[asked[0]] = max(of_steps.get(asked[0], 0), int(asked[1]))
         self.ws = Workspace(rt.device)
-        plans = model.group_plans(cfg.page_size, self._pool_size)
+        plans = model.group_plans(cfg.page_size, partial(self._pool_size, of_steps=sum(of_steps.values())))
         self.cache = CacheManager(plans, model.cache_plan.state_elems, cfg.max_seqs, self.max_seq_len, rt.device,
                                   rt.dtype, cfg.shuffle_pages_seed)
         self.live: Dict[Hashable, LiveRequest] = {}
@@ -194,16 +200,16 @@ class Engine:
         self.last_picks: Optional[torch.Tensor] = None
 
     # ------------------------------------------------------------------ sizing
-    def _pool_size(self, spec, n_layers: int, page_size: int) -> int:
+    def _pool_size(self, spec, n_layers: int, page_size: int, of_steps: int = 0) -> int:
         cfg = self.cfg
         if cfg.num_pages > 0:
             return cfg.num_pages
         if cfg.max_cache_tokens > 0:
             return max(1, -(-cfg.max_cache_tokens // page_size))
-        # from the memory that is free now and that no workspace of the decoding steps will take: every group gets an
+        # from the memory that is free now and that no workspace of the steps will take: every group gets an
         # equal share of the fraction
         free, _ = torch.cuda.mem_get_info(self.rt.device)
-        free = max(0, free - 4 * sum(self._scratch_sizes.values()))
+        free = max(0, free - 4 * (sum(self._scratch_sizes.values()) + of_steps))
         n_groups = max(1, len(self.model.cache_plan.group_specs))
         elem = self.rt.elem_size if spec.dtype is None else torch.empty((), dtype=getattr(torch, spec.dtype)).element_size()
         per_page = n_layers * spec.entries * spec.heads * page_size * spec.head_dim * elem

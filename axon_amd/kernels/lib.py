@@ -1857,11 +1857,14 @@ class Kernels:
             self._check(rc)
         return out
 
+    KV4_CUT = 1 << 14          # segments x heads of cut tiles, at most: of heads of 128 dims each is 68 KB of workspace, together 1.1 GB
+
     def kv4_prefill_tiles(self, spans, window: int, n_heads: int, n_kv_heads: int) -> List[tuple]:
         """The tiles of `kv4_attention_prefill` for portions (first token of the step, tokens, position of the first): rows of (first
         token, count, segment, slot of the workspace), those with the most work first.  A tile whose rows see several segments of positions is
         cut there where a step has few tiles: its segments then run side by side, and are folded behind them.  Rows are of five numbers then,
-        the last of a cut tile's first row its segments, else 0.  The bits are the same either way."""
+        the last of a cut tile's first row its segments, else 0.  The bits are the same either way.  (Tiles with the most work first, as long
+        as cut tiles have no more than `KV4_CUT` segments and heads: `kv4_prefill_most_workspace`.)"""
         tile = int(self.run.axk_kv4_prefill_tile())
         segment_of, start_of = self.run.axk_kv4_prefill_segment, self.run.axk_kv4_prefill_segment_start
         runs = []
@@ -1873,13 +1876,19 @@ class Kernels:
                 runs.append((start + first, n, max(0, at + first + 1 - window) if window > 0 else 0, at + first + n - 1))
         # two workgroups of one head fit a CU: fewer than that, and tiles are cut (a tile at 30,000 positions alone takes 28 of 256 CUs
         # 0.8 ms, and cut 0.2)
-        cut = len(runs) * n_heads < 512
+        ends = [(int(segment_of(low)), int(segment_of(high))) for _, _, low, high in runs]
+        cut, room = set(), self.KV4_CUT // n_heads if len(runs) * n_heads < 512 else 0
+        for i in sorted(range(len(runs)), key=lambda i: runs[i][2] - runs[i][3]):
+            n = ends[i][1] - ends[i][0] + 1
+            if 1 < n <= room:
+                cut.add(i)
+                room -= n
         rows, slots, any_cut = [], 0, 0
-        for start, n, low, high in runs:
-            first, last = int(segment_of(low)), int(segment_of(high))
+        for i, (start, n, low, high) in enumerate(runs):
+            first, last = ends[i]
             if first == last:
                 rows.append((high - low, start, n, -1, -1, 0))
-            elif not cut:
+            elif i not in cut:
                 rows.append((high - low, start, n, -1, slots, 0))
                 slots += 1
             else:
@@ -1889,6 +1898,14 @@ class Kernels:
                 any_cut = 1
         rows.sort(key=lambda r: -r[0])
         return [r[1:5 + any_cut] for r in rows]
+
+    def kv4_prefill_most_workspace(self, max_tokens: int, max_seqs: int, max_seq_len: int, n_heads: int, head_dim: int) -> int:
+        """The most floats that `kv4_prefill_workspace` asks for of a step of up to so many tokens of so many requests."""
+        segments = int(self.run.axk_kv4_prefill_segment(max(0, max_seq_len - 1))) + 1
+        tiles = -(-max_tokens // int(self.run.axk_kv4_prefill_tile())) + max_seqs
+        few = min(tiles, 511 // n_heads)                     # so many may be cut
+        slots = max(min(self.KV4_CUT // n_heads, few * segments) + few, tiles) if segments > 1 else 0
+        return int(self.run.axk_kv4_prefill_workspace(slots, n_heads, head_dim))
 
     @staticmethod
     def kv4_prefill_slots(tiles) -> int:

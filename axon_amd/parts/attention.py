@@ -301,6 +301,12 @@ class GQAttention(Mixer):
             return None
         return ("attention_partial", self.window, self.nh, self.hd), floats
 
+    def step_scratch(self, max_batch_tokens: int, max_seqs: int, max_seq_len: int):
+        if not self.cache_bits:
+            return None
+        floats = self._kernels.kv4_prefill_most_workspace(max_batch_tokens, max_seqs, max_seq_len, self.nh, self.hd)
+        return ("kv4_step", self.window, self.nh, self.nkv, self.hd), floats + KV4_PARTIAL
+
     def load(self, store, rt) -> None:
         self.decode_chunk = rt.k.attention_decode_chunk
         self._work_list = rt.k.attention_decode_work

@@ -226,6 +226,12 @@ class Mixer(Part):
         decoding step and every captured graph then uses the same memory, whatever its shape."""
         return None
 
+    def step_scratch(self, max_batch_tokens: int, max_seqs: int, max_seq_len: int) -> Optional[Tuple[Any, int]]:
+        """(name, float32 elements) of the largest workspace that this mixer takes for a step that feeds prompts and gives back behind
+        it, if it is large, or None.  The engine allocates nothing, but a cache pool that it sizes from the free memory leaves
+        room for it, once per name."""
+        return None
+
     def finishes_following_norm(self, ctx) -> bool:
         """Whether `forward` takes a FollowingNorm as a further argument in this step: its last
         product also writes the finished norm of the rows it has added into.  Optional."""
