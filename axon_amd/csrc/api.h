@@ -545,6 +545,7 @@ int axk_kv4_prefill_tile(void);
 int axk_kv4_prefill_segment(int position);
 int axk_kv4_prefill_segment_start(int segment);
 long axk_kv4_prefill_workspace(int n_slots, int n_heads, int head_dim);
+int axk_kv4_prefill_heads(int n_tiles, int n_heads, int n_kv_heads);       // query heads that a workgroup of such a step takes
 int axk_kv4_attention_prefill(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int32_t* block_table,
                               int table_stride, const int32_t* positions, const int32_t* seq_rows, void* out, const int32_t* tiles,
                               int n_tiles, int columns, float* partial, long partial_floats, int n_heads, int n_kv_heads, int head_dim,

@@ -1081,6 +1081,13 @@ extern "C" long axk_kv4_prefill_workspace(int n_slots, int n_heads, int head_dim
   return (long)n_slots * n_heads * (head_dim == 64 ? Kv4State<64>::FLOATS : Kv4State<128>::FLOATS);
 }
 
+// One query head a workgroup while there are up to three a CU, which spread better; beyond that two, which share what is unpacked: 672
+// tiles and heads in ragged portions 68 against 73 us, 616 of a prompt of 2,800 tokens 103 against 110, 896 of one of 4,096 199 against
+// 190 (28 heads over 4 of 128 dims, the only ones that were timed).  The float32 build has no registers for two.
+extern "C" int axk_kv4_prefill_heads(int n_tiles, int n_heads, int n_kv_heads) {
+  return AXON_BF16 && n_kv_heads > 0 && n_heads / n_kv_heads >= 2 && (long)n_tiles * n_heads > 768 ? 2 : 1;
+}
+
 extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void* k_cache, const void* v_cache,
                                          const int32_t* block_table, int table_stride, const int32_t* positions,
                                          const int32_t* seq_rows, void* out, const int32_t* tiles, int n_tiles, int columns,
@@ -1116,10 +1123,7 @@ extern "C" int axk_kv4_attention_prefill(const void* q, int q_stride, const void
         positions, seq_rows, (elem_t*)out, tiles, columns, partial, n_slots, n_heads, n_kv_heads, page_size, window, scale);    \
   }
 #if AXON_BF16
-  // One query head a workgroup while there are up to three a CU, which spread better; beyond that two, which share what is unpacked: 672
-  // tiles and heads in ragged portions 68 against 73 us, 616 of a prompt of 2,800 tokens 103 against 110, 896 of one of 4,096 199 against
-  // 190.
-  if (group >= 2 && (long)n_tiles * n_heads > 768) {
+  if (axk_kv4_prefill_heads(n_tiles, n_heads, n_kv_heads) == 2) {
     if (head_dim == 64) LAUNCH(64, 2) else LAUNCH(128, 2)
   } else
 #endif

@@ -195,7 +195,7 @@ _PLAIN = ["axk_argmax_workspace", "axk_attention_decode_chunk", "axk_attention_d
           "axk_attention_prefill_tile", "axk_delta_chunked_workspace", "axk_gemm_workspace", "axk_latent_attention_workspace",
           "axk_masked_attention_workspace", "axk_packed_elems", "axk_kv4_decode_chunk", "axk_kv4_decode_item_factor",
           "axk_kv4_decode_workspace", "axk_kv4_prefill_tile", "axk_kv4_prefill_segment",
-          "axk_kv4_prefill_segment_start", "axk_kv4_prefill_workspace"]
+          "axk_kv4_prefill_segment_start", "axk_kv4_prefill_workspace", "axk_kv4_prefill_heads"]
 
 
 def _calls_module():
@@ -1898,6 +1898,10 @@ class Kernels:
                 any_cut = 1
         rows.sort(key=lambda r: -r[0])
         return [r[1:5 + any_cut] for r in rows]
+
+    def kv4_prefill_heads(self, n_tiles: int, n_heads: int, n_kv_heads: int) -> int:
+        """Query heads that a workgroup of `kv4_attention_prefill` takes for so many rows of tiles: 1 or 2, the same bits."""
+        return int(self.run.axk_kv4_prefill_heads(n_tiles, n_heads, n_kv_heads))
 
     def kv4_prefill_most_workspace(self, max_tokens: int, max_seqs: int, max_seq_len: int, n_heads: int, head_dim: int) -> int:
         """The most floats that `kv4_prefill_workspace` asks for of a step of up to so many tokens of so many requests."""

@@ -59,3 +59,18 @@ def test_the_pool_leaves_room_for_them(monkeypatch):
     free = int(((1 << 30) - 4 * (1 << 20)) * 0.85) // per_page
     assert Engine._pool_size(engine, spec, 28, 64) == free
     assert Engine._pool_size(engine, spec, 28, 64, of_steps=1 << 26) == int(((1 << 30) - 4 * (1 << 20) - 4 * (1 << 26)) * 0.85) // per_page < free
+
+
+def test_which_steps_take_two_heads_a_workgroup():
+    """The sizes of the tests that compare one and two heads a workgroup lie on both sides of the rule; the float32 build has one form."""
+    k, f = kernels("bfloat16"), kernels("float32")
+    for nh, nkv, portions in ((14, 2, 57), (28, 4, 29), (9, 3, 90), (5, 1, 160)):        # test_two_heads_a_workgroup
+        assert k.kv4_prefill_heads(portions, nh, nkv) == k.kv4_prefill_heads(1 + 769 // nh + 1, nh, nkv) == 2
+        assert k.kv4_prefill_heads(1, nh, nkv) == f.kv4_prefill_heads(portions, nh, nkv) == 1
+    for nh, nkv, spans, window in ((7, 1, [(300, 5), (130, 0), (77, 1000)], 0), (4, 2, [(257, 700), (64, 64)], 130),
+                                   (3, 1, [(128, 1990), (200, 4000)], 2500)):             # test_one_and_two_heads_a_workgroup_...
+        firsts = [sum(n for n, _ in spans[:i]) for i in range(len(spans))]
+        cut = len(k.kv4_prefill_tiles([(at, n, p) for at, (n, p) in zip(firsts, spans)], window, nh, nkv))
+        whole, nothing = sum(-(-n // 128) for n, _ in spans), 769 // nh + 1
+        assert [k.kv4_prefill_heads(n, nh, nkv) for n in (cut, cut + nothing, whole, whole + nothing)] == [1, 2, 1, 2]
+    assert k.kv4_prefill_heads(65535, 8, 8) == 1                                          # a group of one has no second head
