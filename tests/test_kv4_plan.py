@@ -1,11 +1,12 @@
 """How steps are planned for the 4-bit cache's prompt kernel: the workspace of tiles that are cut has a bound, which a cache pool sized from
-the free memory leaves room for."""
+the free memory leaves room for; which form of the kernel a step takes; and the models that cannot have such a cache."""
+import importlib
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from axon_amd.config import EngineConfig, config_from_dict
+from axon_amd.config import ConfigError, EngineConfig, config_from_dict
 from axon_amd.engine import Engine
 from axon_amd.kernels import kernels
 from axon_amd.models import build_model_description
@@ -74,3 +75,19 @@ def test_which_steps_take_two_heads_a_workgroup():
         whole, nothing = sum(-(-n // 128) for n, _ in spans), 769 // nh + 1
         assert [k.kv4_prefill_heads(n, nh, nkv) for n in (cut, cut + nothing, whole, whole + nothing)] == [1, 2, 1, 2]
     assert k.kv4_prefill_heads(65535, 8, 8) == 1                                          # a group of one has no second head
+
+
+@pytest.mark.parametrize("design", ["pikesun", "figalorn", "napizen", "zugutar", "lilunex", "bafavik"])
+def test_models_whose_mixers_cannot_hold_it_are_refused(design):
+    """By the first mixer that keeps keys and values and has no form for 4 bits, paired ones among them; a model without such a mixer has nothing to
+    hold."""
+    for model in importlib.import_module(f"{design}_models").MODELS.values():
+        config = config_from_dict(model["cfg"])
+        kept = [b.mixer for b in build_model_description(config).blocks if b.mixer.cache_spec() is not None]
+        expect = f"{type(kept[0]).__name__} does not hold its cache in 4 bits" if kept else "no mixer of this model keeps keys and values"
+        with pytest.raises(ConfigError, match=expect):
+            build_model_description(config, 4)
+    for bits in (3, 8):
+        for mixer in kept:
+            with pytest.raises(ConfigError):
+                mixer.hold_cache_in(bits)
