@@ -24,7 +24,7 @@
 #define KV4_COLUMNS 16             // query heads of a key head that a wave takes at a time
 #define KV4_RAISE 8.0f             // how far (log2) scores may pass the reference before it is raised
 #define KV4_WEIGHT 7.0f            // log2 of a weight at the reference: at most 2^15 goes to half precision
-#define KV4_FAR 4096.0f            // references (log2) beyond which scores have theirs taken off before their factor (kv4_offset)
+#define KV4_FAR 4096.0f            // references (log2) beyond which scores have theirs taken off before their factor (kv4_refer)
 #define LOG2E 1.4426950408889634f
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -80,26 +80,29 @@ __host__ __device__ inline int kv4_chunk(int seen) {
   return rounds * KV4_WAVES * KV4_BLOCK;
 }
 
-// The weights are taken relative to a reference, a score as the products leave it (times c: its log2), which is raised to a block's maximum
-// only where that is KV4_RAISE or more above it (the first block's always): what was summed before is then scaled by the factor
-// returned, 1 for a column whose reference stays.  A column's arithmetic depends on its own scores alone.
-__device__ __forceinline__ float kv4_raise(float& ref, float block_max, float c) {
-  const bool up = __fmul_rn(__fsub_rn(block_max, ref), c) > KV4_RAISE;        // (nothing seen yet, and nothing now: not a number, so no)
-  const float before = ref;
-  ref = up ? block_max : ref;
-  return up ? __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(before, ref), c)) : 1.0f;
+// The weights are taken relative to a reference, which is raised to a block's maximum only where that is KV4_RAISE or more above it
+// (the first block's always): what was summed before is then scaled by the factor returned, 1 for a column whose
+// reference stays.  A column's arithmetic depends on its own scores alone.
+struct Kv4Reference {
+  float score = -INFINITY;         // as the products leave it; times c its log2
+  float add = 0.0f;                // what a score times c has added to it for its weight's log2
+  bool far = false;                // a column of the wave has its reference taken off its scores
+};
+__device__ __forceinline__ float kv4_raise(Kv4Reference& ref, float block_max, float c) {
+  const bool up = __fmul_rn(__fsub_rn(block_max, ref.score), c) > KV4_RAISE;  // (nothing seen yet, and nothing now: not a number, so no)
+  const float before = ref.score;
+  ref.score = up ? block_max : before;
+  return up ? __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(before, ref.score), c)) : 1.0f;
 }
 
-// What a score s c has added to it for its weight's log2.  ref c rounded and KV4_WEIGHT less that rounded are off by 2^-13 each up to KV4_FAR,
+// The rest of it, where one of the wave's was raised.  score c rounded and KV4_WEIGHT less that rounded are off by 2^-13 each up to KV4_FAR,
 // for all of a reference's weights alike.  At 2^25 they would be off by more than KV4_WEIGHT, and weights out of half precision's range:
-// a column beyond KV4_FAR has its reference taken off its scores instead (subtract(reference), which is 0 for the wave's other
-// columns and leaves them as they are), exactly where it matters, near the largest.
-template <typename Subtract>
-__device__ __forceinline__ float kv4_offset(float ref, float c, Subtract subtract) {
-  const float at = __fmul_rn(ref, c);
-  const bool far = fabsf(at) > KV4_FAR && fabsf(ref) < INFINITY;
-  if (__any(far)) subtract(far ? ref : 0.0f);
-  return ref == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, far ? 0.0f : at);
+// a column beyond KV4_FAR has its reference taken off its scores before their factor, exactly where it matters, near the largest.
+__device__ __forceinline__ bool kv4_far(float score, float c) { return fabsf(__fmul_rn(score, c)) > KV4_FAR && fabsf(score) < INFINITY; }
+__device__ __forceinline__ void kv4_refer(Kv4Reference& ref, float c) {
+  const bool far = kv4_far(ref.score, c);
+  ref.far = __any(far);
+  ref.add = ref.score == -INFINITY ? 0.0f : __fsub_rn(KV4_WEIGHT, far ? 0.0f : __fmul_rn(ref.score, c));
 }
 
 // ============================================================================ single tokens
@@ -205,7 +208,7 @@ __device__ __forceinline__ void kv4_scores(const Kv4Keys<HD>& keys, const u32x4 
 // seen (the same for the wave); else those of lo .. pos are, and the block begins at p0.  rescale(factor) is called where a reference of
 // the wave is raised.
 template <typename Rescale>
-__device__ __forceinline__ void kv4_weights(f32x4 (&s)[4], bool whole, int p0, int lo, int pos, float c, int lane, float& ref, float& l,
+__device__ __forceinline__ void kv4_weights(f32x4 (&s)[4], bool whole, int p0, int lo, int pos, float c, int lane, Kv4Reference& ref, float& l,
                                             u32x4 (&pf)[2][TERMS], Rescale rescale) {
   if (!whole) {
     int first = p0 + 8 * (lane >> 4);
@@ -229,20 +232,22 @@ __device__ __forceinline__ void kv4_weights(f32x4 (&s)[4], bool whole, int p0, i
   if (__any(factor != 1.0f)) {
     l = __fmul_rn(l, factor);
     rescale(factor);
+    kv4_refer(ref, c);
   }
-  const float add = kv4_offset(ref, c, [&](float off) {
+  if (__builtin_expect(ref.far, 0)) {
+    const float off = kv4_far(ref.score, c) ? ref.score : 0.0f;                // (0 leaves a score as it is)
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[t][r] = __fsub_rn(s[t][r], off);
-  });
+  }
   float sum = 0.0f;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     float w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + (i >> 2)][i & 3], c, add));
+      w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * u + (i >> 2)][i & 3], c, ref.add));
       sum = __fadd_rn(sum, w[i]);
     }
     kv4_split(w, pf[u]);
@@ -367,7 +372,8 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
                                        page_size, lane);
   __shared__ __align__(16) float o_of[KV4_WAVES][KV4_COLUMNS][HD + 4];
   __shared__ float ref_of[KV4_WAVES][KV4_COLUMNS], l_of[KV4_WAVES][KV4_COLUMNS];
-  float ref = -INFINITY, l = 0.0f;
+  Kv4Reference ref;
+  float top_log2 = -INFINITY, l = 0.0f;              // (what is joined is compared as log2)
   f32x4 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -402,7 +408,7 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
     }
     l = __fadd_rn(l, __shfl_xor(l, 16, AXON_WAVE));
     l = __fadd_rn(l, __shfl_xor(l, 32, AXON_WAVE));
-    ref = __fmul_rn(ref, c);                   // (what is joined is compared as log2)
+    top_log2 = __fmul_rn(ref.score, c);
   }
   if (l16 < columns) {
 #pragma unroll
@@ -411,7 +417,7 @@ kv4_decode_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned cha
       for (int dt = 0; dt < DT; dt += 4)
         *reinterpret_cast<float4*>(&o_of[wave][l16][DT * (4 * h + r) + dt]) = make_float4(o[dt][r], o[dt + 1][r], o[dt + 2][r], o[dt + 3][r]);
     if (h == 0) {
-      ref_of[wave][l16] = ref;
+      ref_of[wave][l16] = top_log2;
       l_of[wave][l16] = l;
     }
   }
@@ -792,13 +798,14 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   }
   Kv4State<HD> st;
   f32x16(&o)[DT] = st.o;
-  float &ref = st.ref, &l = st.l;
+  float& l = st.l;
+  Kv4Reference ref;
   auto clear = [&]() {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-    ref = -INFINITY;
+    ref = Kv4Reference{};
     l = 0.0f;
   };
 
@@ -902,13 +909,15 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[dt][e] = __fmul_rn(o[dt][e], factor);
+        kv4_refer(ref, c);
       }
-      const float add = kv4_offset(ref, c, [&](float off) {
+      if (__builtin_expect(ref.far, 0)) {
+        const float off = kv4_far(ref.score, c) ? ref.score : 0.0f;
 #pragma unroll
         for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[pt][e] = __fsub_rn(s[pt][e], off);
-      });
+      }
       // The weights of sixteen positions, then their products with all dims: on those the matrix cores work while the vector unit has the
       // weights of the next sixteen.
       float sum[2] = {0.0f, 0.0f};
@@ -925,7 +934,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
         u32x4 pf[TERMS];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], c, add));
+          w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st >> 1][8 * (st & 1) + i], c, ref.add));
           sum[i & 1] = __fadd_rn(sum[i & 1], w[i]);
         }
         asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));       // (added here, beside products: else behind the last of them, 1 to 2 % later)
@@ -951,7 +960,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
   }
   for (; b < seg_end; ++b) pass(b);
   if (!live || (segment < 0 && seg_first == seg_last)) continue;
-  ref = __fmul_rn(ref, c);                         // (what is folded is compared as log2)
+  st.ref = __fmul_rn(ref.score, c);                // (what is folded is compared as log2)
   if (kept) kv4_fold<HD, true>(st, state_at, wave & 3, lane, 0);
   if (seg_end < n_blocks || segment >= 0) {
     kv4_store<HD>(st, state_at, wave & 3, lane, nan_groups);
@@ -965,7 +974,7 @@ __device__ __forceinline__ void kv4_prefill_tile(unsigned char* smem, int t0, in
 
 // tiles [n][columns] = (first token, count, segment or -1 for all that the tile sees, slot of the workspace, kv4_fold_kernel's).
 template <int HD, int HPB>
-__global__ void __launch_bounds__(256 * HPB, TERMS == 1 ? 2 : 1)
+__global__ void __launch_bounds__(256 * HPB, TERMS == 1 || HD == 64 ? 2 : 1)
 kv4_prefill_kernel(const elem_t* __restrict__ q, int q_stride, const unsigned char* __restrict__ k_cache,
                    const unsigned char* __restrict__ v_cache, const int32_t* __restrict__ block_table, int table_stride,
                    const int32_t* __restrict__ positions, const int32_t* __restrict__ seq_rows, elem_t* __restrict__ out,
