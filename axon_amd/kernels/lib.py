@@ -1829,8 +1829,8 @@ class Kernels:
     def kv4_attention_decode(self, q, q_stride, k_cache, v_cache, block_table, positions, seq_rows, out, token_index, partial,
                              max_chunks, n_heads, n_kv_heads, head_dim, page_size, window, scale, work) -> torch.Tensor:
         """`attention_decode` over a cache held in 4 bits: tokens named by token_index (int32), or the first `token_index` of the
-        step.  `work` (int32, on the device): `kv4_decode_work` of their positions, -1 for nothing; partial: float32,
-        `kv4_decode_workspace`."""
+        step.  `work` (int32, on the device): `kv4_decode_work` of their positions, -1 for nothing; max_chunks: `kv4_decode_chunks` of them at
+        least (chunks beyond it are left out); partial: float32, `kv4_decode_workspace`."""
         what = "kv4_attention_decode"
         T, stream = self._kv4_step(what, k_cache, v_cache, block_table, positions, seq_rows, n_kv_heads, head_dim, page_size, q, out, partial,
                                    work)

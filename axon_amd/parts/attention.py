@@ -407,7 +407,8 @@ class GQAttention(Mixer):
                                                  and k.gemm_qkv_rope_ok(T, width, self.hidden, self.hd, self.hd)):
             h = h.apply(ctx)
         if isinstance(h, PrecedingNorm):
-            # Few rows: the norm and the product in one launch, every head a query's that turns by an angle of zero (x 1 - y 0 is x).  The
+            # Few rows: the norm and the product in one launch, every head a query's that turns by an angle of zero (x 1 - y 0 is x; a
+            # projection that is beyond the type's range, and so not finite, has its pair not a number too).  The
             # rotation is the next kernel's, which quantises keys that were not rounded behind it.
             k.gemm_normed_qkv_rope(h.rows, h.gain, h.eps, w, bias, qkv, self.unturned[:T], ctx.positions, ctx.seq_rows, group.block_table,
                                    None, None, width // self.hd, self.nkv, self.hd, group.page_size, False)
