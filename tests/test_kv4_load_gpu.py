@@ -1,5 +1,7 @@
 """Generation with keys and values held in 4 bits under load: a request's tokens are those that it gets alone, whatever other requests leave
 of a step's tokens and of the pages: prompts cut anywhere (into portions of one token too), requests that give way and are fed again."""
+import random
+
 import pytest
 import torch
 
@@ -7,7 +9,7 @@ import axon_amd
 from axon_amd.engine import StepEntry, StepError
 from axon_amd.parts import attention
 from gpu_helpers import DTYPES
-from helpers import TINY, prompts_for
+from helpers import TINY, prompts_for, run_trace
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +82,33 @@ def test_steps_that_are_told_the_prompts_tokens(model_dirs, monkeypatch, dtype, 
         assert torch.equal(llm.engine.step([StepEntry("r", [ids[i]], [0])], end=["r"] if i == 92 else []), want[i:i + 1])
     assert torch.equal(llm.logits(ids[:1]), llm.logits(ids[:1], all_positions=True)[0])
     assert torch.equal(llm.logits(ids[:1]), want[0])
+
+
+def test_the_trace_program_is_told_them_too(model_dirs, tmp_path):
+    d = model_dirs("D", "bfloat16")
+    ids = prompts_for("D", (22,), seed=4)[0]
+    llm = axon_amd.load(d, cache_bits=4, page_size=16, num_pages=16, max_seqs=2)
+    want = llm.logits(ids, all_positions=True).cpu().numpy()
+    steps = [{"step": 0, "entries": [{"id": "a", "tokens": ids[:20], "want": [19]}], "end": []},
+             {"step": 1, "entries": [{"id": "a", "tokens": ids[20:21], "want": [0], "prompt": 1}], "end": []},
+             {"step": 2, "entries": [{"id": "a", "tokens": ids[21:], "want": [0], "prompt": 1}], "end": ["a"]}]
+    got = run_trace(d, "bfloat16", steps, str(tmp_path), 64, ["--cache-bits", "4"])
+    assert all((got[i][0] == want[19 + i]).all() for i in range(3))
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_loads(model_dirs, seed):
+    """Requests of random lengths under a random budget and too few pages: what each gets alone."""
+    rng = random.Random(seed)
+    name = rng.choice("DE")
+    d = model_dirs(name, "bfloat16")
+    prompts = prompts_for(name, [rng.choice([1, 2, 5, 16, 17, 40, 90, 130]) for _ in range(7)], seed=seed)
+    page, kw = rng.choice([8, 16, 64]), dict(max_new_tokens=rng.choice([9, 30]))
+    if rng.random() < 0.5:
+        kw.update(temperature=0.8, seed=seed)
+    roomy = axon_amd.load(d, cache_bits=4, page_size=page, num_pages=7 * (170 // page + 2), max_seqs=7)
+    want = roomy.generate(prompts, **kw)
+    assert roomy.last_stats.preemptions == 0
+    tight = axon_amd.load(d, cache_bits=4, page_size=page, num_pages=170 // page + 2, max_seqs=5, max_batch_tokens=rng.choice([3, 18, 50, 200]),
+                          use_graphs=rng.random() < 0.5)
+    assert tight.generate(prompts, **kw) == want
